@@ -343,7 +343,7 @@ def run(s):
         k, v = p8.read_paged8_cache(*cache, cu_seqlens=s["cu"], num_tokens=s["total"], dtype=DTYPES[s["dtype"]],
                                     kv_layout=s["layout"])
         return [k, v]
-    return p8.paged8_attention(s["q"], *cache, cu_seqlens=s["cu"], max_seq_len=s["longest"], sm_scale=SCALE,
+    return p8.paged8_attention(s["q"], *cache, cu_seqlens=s["cu"], sm_scale=SCALE,
                                window=s["window"] or None, sink=SINK if s["window"] else 0, kv_layout=s["layout"])
 
 
