@@ -31,6 +31,7 @@ LIB_PATH = os.path.join(_HERE, _LIBRARIES[_which])
 
 # element types / layouts / workspace kinds (include/kvdec.h)
 F16, F32, BF16 = 0, 1, 2
+I8, E4M3 = 3, 4   # code types (include/kvdec_paged8.h)
 LAYOUT_LINEAR, LAYOUT_RING = 0, 1
 KIND_DENSE, KIND_SPARSE, KIND_KIVI, KIND_KIVI_SPLIT = 0, 1, 2, 3
 
@@ -95,13 +96,32 @@ SIGNATURES = {
 }
 
 
+class Paged8Cache(ctypes.Structure):
+    """kvdec_paged8_cache (include/kvdec_paged8.h)."""
+    _fields_ = ([(n, _vp) for n in ("k_pages", "v_pages", "k_scales", "v_scales", "block_table", "seq_lens")]
+                + [(n, _i64) for n in ("num_pages", "page_stride", "row_stride", "head_stride")]
+                + [(n, _i32) for n in ("code", "KVH", "D", "page_size", "block_size", "max_blocks")])
+
+
+# every symbol include/kvdec_paged8.h declares
+PAGED8_SIGNATURES = {
+    "kvdec_paged8_write": (ctypes.c_int, [ctypes.POINTER(Paged8Cache), _vp, _vp, ctypes.c_int, _i64, _i64, _i64,
+                                          _i64, _vp, _i64, _i64, _vp]),
+    "kvdec_paged8_read": (ctypes.c_int, [ctypes.POINTER(Paged8Cache), _vp, _i64, _i64, _vp, _vp, ctypes.c_int,
+                                         _vp]),
+    "kvdec_paged8_attention": (ctypes.c_int, [ctypes.POINTER(Paged8Cache), _vp, _vp, ctypes.c_int, _i64, _i64, _vp,
+                                              _i64, _i64, _i32, _i32, _i32, _f32, _vp, _sz, _vp]),
+    "kvdec_paged8_workspace_bytes": (_sz, [_i64, _i64, _i32, _i32, _i64]),
+}
+
+
 def _load() -> ctypes.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
             f"{LIB_PATH} is missing: build it with `python {os.path.join(_HERE, 'build.py')}` "
             "(or __graft_entry__.build()); there is no CPU fallback")
     lib = ctypes.CDLL(LIB_PATH)
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in {**SIGNATURES, **PAGED8_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

@@ -36,6 +36,7 @@ SOURCES = (
     ("attn.hip", []),
     ("quant.hip", ["-ffp-contract=off"]),
     ("generic.hip", []),
+    ("paged8.hip", []),
 )
 CLOCK_LIB_PATH = os.path.join(HERE, "libkvdec_clock.so")
 # object name, source, extra flags; each library links the objects it names
@@ -44,11 +45,12 @@ OBJECTS = (
     ("attn_clock", "attn.hip", ["-DKVDEC_CLOCK"]),
     ("quant", "quant.hip", ["-ffp-contract=off"]),
     ("generic", "generic.hip", []),
+    ("paged8", "paged8.hip", []),
 )
 HOST_LIB_PATH = os.path.join(HERE, "_kvdec_host.so")
 LIBRARIES = (
-    (LIB_PATH, ("attn", "quant", "generic")),
-    (CLOCK_LIB_PATH, ("attn_clock", "quant", "generic")),
+    (LIB_PATH, ("attn", "quant", "generic", "paged8")),
+    (CLOCK_LIB_PATH, ("attn_clock", "quant", "generic", "paged8")),
 )
 
 COMMON_FLAGS = [

@@ -15,9 +15,11 @@
 
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/TracerMode.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/generated/variable_factories.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -28,6 +30,7 @@
 #include <initializer_list>
 
 #include "kvdec.h"
+#include "kvdec_paged8.h"
 
 namespace {
 
@@ -38,7 +41,8 @@ using Shape = std::initializer_list<int64_t>;
   X(kvdec_workspace_bytes) X(kvdec_dense_decode) X(kvdec_sparse_decode) X(kvdec_paged_decode)    \
   X(kvdec_sparse_decode_varlen) X(kvdec_quantize_k) X(kvdec_quantize_v) X(kvdec_sparse_decode_kivi) \
   X(kvdec_sparse_decode_kivi_varlen) X(kvdec_sparse_decode_kivi_typed) X(kvdec_build_kivi_cache) \
-  X(kvdec_kivi_stream_step_decode)
+  X(kvdec_kivi_stream_step_decode) X(kvdec_paged8_write) X(kvdec_paged8_read) X(kvdec_paged8_attention)    \
+  X(kvdec_paged8_workspace_bytes)
 
 // The library's entry points, resolved once by bind().
 struct Lib {
@@ -469,6 +473,145 @@ PyObject* build(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// -- paged 8-bit cache ----------------------------------------------------------
+
+// The cache's seven tensors (k_pages, v_pages, k_scales, v_scales, block_table,
+// seq_lens, cu_seqlens or None) and its layout.
+struct Paged8 {
+  kvdec_paged8_cache c{};
+  const Tensor* k = nullptr;
+  const int32_t* cu = nullptr;
+  int64_t B = 0;
+
+  bool parse(PyObject* const* a, PyObject* layout) {
+    const Tensor *v, *ks, *vs, *table, *lens;
+    if (!PyUnicode_Check(layout)) return false;
+    const bool hnd = PyUnicode_CompareWithASCIIString(layout, "HND") == 0;
+    if (!hnd && PyUnicode_CompareWithASCIIString(layout, "NHD") != 0) return false;
+    if (!(k = gpu_tensor(a[0])) || !(v = gpu_tensor(a[1])) || !(ks = gpu_tensor(a[2])) || !(table = gpu_tensor(a[4])) ||
+        k->dim() != 4 || ks->dim() != 3 || table->dim() != 2)
+      return false;
+    const at::ScalarType type = k->scalar_type();
+    const c10::Device dev = k->device();
+    const int rows = hnd ? 2 : 1, heads = hnd ? 1 : 2;
+    const int64_t pages = k->size(0), KVH = k->size(heads), ps = k->size(rows), blocks = ks->size(2);
+    B = table->size(0);
+    if ((type != at::kChar && type != at::kFloat8_e4m3fn) || v->scalar_type() != type || v->device() != dev ||
+        k->sizes() != v->sizes() || k->strides() != v->strides() || k->stride(3) != 1 || k->size(3) != 128 ||
+        !fits_i32(KVH) || !fits_i32(ps) || ps < 16 || blocks < 1 || ps % blocks || !fits_i32(table->size(1)))
+      return false;
+    if (!(ks = exactly(a[2], at::kFloat, {pages, KVH, blocks}, dev)) ||
+        !(vs = exactly(a[3], at::kFloat, {pages, KVH, blocks}, dev)) ||
+        !(table = exactly(a[4], at::kInt, {B, table->size(1)}, dev)) || !(lens = exactly(a[5], at::kInt, {B}, dev)))
+      return false;
+    if (a[6] != Py_None) {
+      const Tensor* t = exactly(a[6], at::kInt, {B + 1}, dev);
+      if (!t) return false;
+      cu = (const int32_t*)t->data_ptr();
+    }
+    c = {k->data_ptr(), v->data_ptr(), (float*)ks->data_ptr(), (float*)vs->data_ptr(),
+         (const int32_t*)table->data_ptr(), (const int32_t*)lens->data_ptr(), pages, k->stride(0), k->stride(rows),
+         k->stride(heads), type == at::kChar ? KVDEC_I8 : KVDEC_E4M3, (int32_t)KVH, 128, (int32_t)ps,
+         (int32_t)(ps / blocks), (int32_t)table->size(1)};
+    return B > 0;
+  }
+
+  // New tokens' rows: [T, heads, 128] of a type, on 16-byte boundaries.
+  const Tensor* rows(PyObject* o, int64_t heads, at::ScalarType type) const {
+    const Tensor* x = gpu_tensor(o);
+    if (!x || x->dim() != 3 || x->scalar_type() != type || elt(*x) < 0 || x->device() != k->device() ||
+        x->size(1) != heads || x->size(2) != 128 || x->stride(2) != 1 || x->size(0) < 1 || (!cu && x->size(0) != B))
+      return nullptr;
+    const int64_t per16 = 16 / x->element_size();
+    return (uintptr_t)x->data_ptr() % 16 || x->stride(0) % per16 || x->stride(1) % per16 ? nullptr : x;
+  }
+};
+
+// paged8_write(k, v, cache's seven, layout)
+PyObject* paged8_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Paged8 p;
+  const Tensor *k, *v;
+  if (n != 10 || !plain_mode() || !p.parse(a + 2, a[9]) || !(k = gpu_tensor(a[0])) ||
+      !(k = p.rows(a[0], p.c.KVH, k->scalar_type())) || !(v = p.rows(a[1], p.c.KVH, k->scalar_type())) ||
+      v->size(0) != k->size(0))
+    return none();
+  int rc;
+  {
+    NoGil no_gil;
+    const c10::DeviceGuard guard(k->device());
+    rc = lib.kvdec_paged8_write(&p.c, k->data_ptr(), v->data_ptr(), elt(*k), k->stride(0), k->stride(1), v->stride(0),
+                                v->stride(1), p.cu, p.B, k->size(0), stream(*k));
+  }
+  if (rc == 0) Py_RETURN_TRUE;
+  Tensor unused;
+  return done(rc, "write_paged8_cache", unused);
+  END_HANDLE_TH_ERRORS
+}
+
+// paged8_read(cache's seven, num_tokens, dtype, layout)
+PyObject* paged8_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Paged8 p;
+  int64_t T;
+  if (n != 10 || !plain_mode() || !p.parse(a, a[9]) || !THPDtype_Check(a[8])) return none();
+  if (a[7] == Py_None && !p.cu)
+    T = p.B;
+  else if (!to_i64(a[7], T) || T < 1 || (!p.cu && T != p.B))
+    return none();
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(a[8])->scalar_type;
+  if (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat) return none();
+  Tensor out[2];
+  int rc;
+  {
+    NoGil no_gil;
+    const c10::DeviceGuard guard(p.k->device());
+    for (Tensor& o : out) o = empty({T, p.c.KVH, 128}, *p.k, type);
+    rc = lib.kvdec_paged8_read(&p.c, p.cu, p.B, T, out[0].data_ptr(), out[1].data_ptr(), elt(out[0]), stream(*p.k));
+  }
+  if (rc) return done(rc, "read_paged8_cache", out[0]);
+  PyObject* r = PyTuple_New(2);
+  for (int i = 0; r && i < 2; ++i) {
+    PyObject* t = THPVariable_Wrap(std::move(out[i]));
+    if (!t) {
+      Py_DECREF(r);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(r, i, t);
+  }
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged8_attention(q, cache's seven, sm_scale, window, sink, layout)
+PyObject* paged8_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Paged8 p;
+  float scale;
+  int32_t window = 0, sink;
+  const Tensor* q;
+  if (n != 12 || !plain_mode() || !p.parse(a + 1, a[11]) || !(q = gpu_tensor(a[0])) || q->dim() != 3 ||
+      !(q = p.rows(a[0], q->size(1), q->scalar_type())) || elt(*q) == KVDEC_F32 || !fits_i32(q->size(1)) ||
+      q->size(1) < 1 || q->size(1) % p.c.KVH || !to_f32(a[8], scale) || !to_i32(a[10], sink) || sink < 0 ||
+      (a[9] == Py_None ? sink > 0 : !to_i32(a[9], window) || window < 1))
+    return none();
+  const int64_t T = q->size(0), H = q->size(1);
+  Tensor o;
+  int rc;
+  {
+    NoGil no_gil;
+    const c10::DeviceGuard guard(q->device());
+    o = empty({T, H, 128}, *q, q->scalar_type());
+    const size_t bytes =
+        lib.kvdec_paged8_workspace_bytes(p.B, T, (int)H, p.c.KVH, (int64_t)p.c.max_blocks * p.c.page_size);
+    const Tensor ws = workspace(bytes, *q);
+    rc = lib.kvdec_paged8_attention(&p.c, q->data_ptr(), o.data_ptr(), elt(*q), q->stride(0), q->stride(1), p.cu, p.B, T,
+                                    (int)H, window, sink, scale, ptr(ws), bytes, stream(*q));
+  }
+  return done(rc, "paged8_attention", o);
+  END_HANDLE_TH_ERRORS
+}
+
 // -- module ---------------------------------------------------------------------
 
 // bind(path, check): the loaded libkvdec.so and _kvdec.check.
@@ -493,7 +636,8 @@ PyObject* bind(PyObject*, PyObject* args) {
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, nullptr},
     KVDEC_FAST(sparse), KVDEC_FAST(dense), KVDEC_FAST(paged), KVDEC_FAST(kivi), KVDEC_FAST(step_attend),
-    KVDEC_FAST(quantize), KVDEC_FAST(build), {nullptr, nullptr, 0, nullptr}};
+    KVDEC_FAST(quantize), KVDEC_FAST(build), KVDEC_FAST(paged8_write), KVDEC_FAST(paged8_read),
+    KVDEC_FAST(paged8_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kvdec_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
