@@ -408,14 +408,10 @@ __global__ __launch_bounds__(64 * kWriteWaves) void read8_kernel(Read8Args A) {
 // ---------------------------------------------------------------------------
 //
 // The query rows of a sequence and KV head are its new tokens' heads of the
-// group, token-major: row r is head r % G of new token r / G.  A unit is
-// kRowsA of them (the columns of the matrix instruction); unit and KV head
-// make a pair, whose keys come in tiles of 32 tokens.
-//
-// The tiles of all pairs, in order, are dealt to the launch's workgroups in
-// equal runs, whatever the sequences' lengths: each finds its run from the
-// lengths on the device.  A pair that falls to several workgroups leaves
-// partial rows in the workspace, which a second kernel joins.
+// group, token-major: row r is head r % G of new token r / G.  Sequences of at
+// most kRowsA rows (single tokens, mostly) are read by the narrow kernel, whose
+// work is the reading of the cache, those of more by the wide one, whose work
+// is the products.
 //
 // Softmax over scaled codes.  With x = log2(e) sm_scale (q . k) per token, the
 // scale of V's block enters as x + log2(vs): w = exp2(x + log2(vs) - m) is the
@@ -430,15 +426,21 @@ constexpr int kSlotA = 2 * kTile * kCodeRow;        // K and V codes of a tile
 constexpr int kGroupsA = 1024;                      // workgroups of a launch, at most
 static_assert(kRowsA * kHeadDim * 4 <= kSlotA, "a wave's partial rows fit its slot");
 
+constexpr int kRowsB = 128;                         // query rows of a workgroup, 32 a wave
+constexpr int kThreadsB = 256;
+constexpr int kTileB = 64;                          // tokens of its tiles
+constexpr int kPairsB = 512;                        // workgroups that fill the GPU
+
 struct Attn8Args {
   Cache8 C;
   const void* q;
   void* o;
-  float* part;                // [2 * groups][kRowsA][128], then maxima and sums
+  float* part;                // partial rows, then their maxima and sums
   int64_t q_tok, q_head;      // in elements
   int64_t units;
   int32_t G, H, window, sink;
-  int32_t groups;
+  int32_t groups;             // narrow: workgroups
+  int32_t splits;             // wide: workgroups a pair
   float scale_log2;
 };
 
@@ -452,37 +454,113 @@ struct Unit8 {
   __device__ __forceinline__ int tile(int j) const { return j < ts ? j : tw + j - ts; }
 };
 
-__device__ __forceinline__ Unit8 unit8(const Attn8Args& A, int64_t u) {
-  const Cache8& C = A.C;
-  Unit8 U;
-  int64_t b;
-  if (C.cu == nullptr) {
-    const int per = (A.G + kRowsA - 1) / kRowsA;
-    b = u / per;
-    U.row0 = (int)(u - b * per) * kRowsA;
-  } else {
-    auto first = [&](int64_t s) { return (int64_t)offset8(C, s) * A.G / kRowsA + s; };
-    b = seq_of_unit(C.B, u, first);
-    U.row0 = (int)min((u - first(b)) * kRowsA, (int64_t)1 << 30);
-  }
-  U.s = seq8(C, b);
-  U.rows = (int)min((int64_t)U.s.n * A.G - U.row0, (int64_t)kRowsA);
+template <int TILE>
+__device__ __forceinline__ void unit_tiles(const Attn8Args& A, Unit8& U) {
   U.ts = U.tw = U.te = 0;
   U.pos0 = U.pos1 = -1;
   if (U.rows <= 0) {
     U.rows = 0;
-    return U;
+    return;
   }
   U.pos0 = U.s.len - U.s.n + U.row0 / A.G;
   U.pos1 = U.s.len - U.s.n + (U.row0 + U.rows - 1) / A.G;
-  if (U.pos1 < 0) return U;
-  U.te = U.pos1 / kTile + 1;
+  if (U.pos1 < 0) return;
+  U.te = U.pos1 / TILE + 1;
   if (A.window > 0) {
-    U.ts = min((int)(((int64_t)A.sink + kTile - 1) / kTile), U.te);
-    U.tw = min(max(U.ts, max(U.pos0 - A.window + 1, 0) / kTile), U.te);
+    U.ts = min((int)(((int64_t)A.sink + TILE - 1) / TILE), U.te);
+    U.tw = min(max(U.ts, max(U.pos0 - A.window + 1, 0) / TILE), U.te);
   }
+}
+
+// The narrow kernel's unit: a sequence, if its rows fit.
+__device__ __forceinline__ Unit8 unit_a(const Attn8Args& A, int64_t b) {
+  Unit8 U;
+  U.s = seq8(A.C, b);
+  const int64_t rows = (int64_t)U.s.n * A.G;
+  U.row0 = 0;
+  U.rows = rows <= kRowsA ? (int)rows : 0;
+  unit_tiles<kTile>(A, U);
   return U;
 }
+
+// The wide kernel's unit u: kRowsB rows of a sequence of more than kRowsA, or of
+// the rows past the last sequence (which attend to nothing).
+__device__ __forceinline__ Unit8 unit_b(const Attn8Args& A, int64_t u) {
+  const Cache8& C = A.C;
+  Unit8 U;
+  int64_t b, first;
+  if (C.cu == nullptr) {
+    const int per = (A.G + kRowsB - 1) / kRowsB;
+    b = u / per;
+    first = b * per;
+  } else {
+    auto start = [&](int64_t s) { return (int64_t)offset8(C, s) * A.G / kRowsB + s; };
+    b = seq_of_unit(C.B, u, start);
+    first = start(b);
+  }
+  U.s = seq8(C, b);
+  const int64_t rows = (int64_t)U.s.n * A.G, row0 = (u - first) * kRowsB;
+  U.row0 = (int)min(row0, rows);
+  U.rows = rows > kRowsA || b == C.B ? (int)min(rows - U.row0, (int64_t)kRowsB) : 0;
+  unit_tiles<kTileB>(A, U);
+  return U;
+}
+
+// Where a token of a tile stands against a row's position.
+__device__ __forceinline__ bool sees(int p, int pos, int window, int sink) {
+  return p <= pos && (window <= 0 || p < sink || p > pos - window);
+}
+
+// Every token of [tok, tok + n) is seen by every row of the unit.
+__device__ __forceinline__ bool all_seen(const Attn8Args& A, const Unit8& U, int tok, int n) {
+  return tok + n - 1 <= U.pos0 && (A.window <= 0 || tok + n <= A.sink || tok > U.pos1 - A.window);
+}
+
+// What a token of the pair's rows weighs by: kf turns q . k into x, lv is
+// log2 of V's scale and inv its inverse.  No page: keys and values of zero.
+struct Meta8 {
+  int page;
+  float kf, lv, inv;
+};
+
+__device__ __forceinline__ Meta8 meta8(const Attn8Args& A, int b, int head, int tok, bool live) {
+  const Cache8& C = A.C;
+  Meta8 m = {-1, 0.f, 0.f, 1.f};
+  if (live) {
+    const int id = C.bt[(int64_t)b * C.max_blocks + (tok >> C.ps_log2)];
+    if (id >= 0 && id < C.num_pages) {
+      m.page = id;
+      const int64_t at = scale_index(C, id, head, tok);
+      m.kf = C.ks[at] * A.scale_log2;
+      const float vs = C.vs[at];
+      // a scale that is hardly one counts as the writer's least
+      const float s = vs < 0x1p-100f ? 0x1p-100f : vs;
+      m.lv = __builtin_amdgcn_logf(s);
+      m.inv = s == s ? 1.f / s : 1.f;   // a NaN arrives through lv, where masks hold
+    }
+  }
+  return m;
+}
+
+// Place of row `row` of a pair in the output.
+__device__ __forceinline__ int64_t out_row(const Attn8Args& A, const Unit8& U, int head, int row) {
+  const int r = U.row0 + row, tok = r / A.G;
+  return ((int64_t)(U.s.c0 + tok) * A.H + head * A.G + (r - tok * A.G)) * kHeadDim;
+}
+
+template <int E>
+__device__ __forceinline__ void store_out(const Attn8Args& A, int64_t at, float4v acc, float l) {
+  const float d = l == 0.f ? 1.f : l;
+  *reinterpret_cast<u32x2*>((uint16_t*)A.o + at) = round_elt4<E>(float4v{acc[0] / d, acc[1] / d, acc[2] / d, acc[3] / d});
+}
+
+// ---- the narrow kernel ----
+//
+// The tiles (32 tokens) of all pairs of a sequence and a KV head, in order, are
+// dealt to the launch's workgroups in equal runs, whatever the sequences'
+// lengths: each finds its run from the lengths on the device.  A pair that
+// falls to several workgroups leaves partial rows in the workspace, which a
+// second kernel joins.
 
 __device__ __forceinline__ uint32_t wave_total(uint32_t x) {
 #pragma unroll
@@ -490,15 +568,15 @@ __device__ __forceinline__ uint32_t wave_total(uint32_t x) {
   return __builtin_amdgcn_readfirstlane(x);
 }
 
-// Tiles of all units, and of those before unit u (one KV head's).
+// Tiles of all sequences, and of those before sequence u (one KV head's).
 struct Counts8 {
   int64_t all, before;
 };
 __device__ __forceinline__ Counts8 count8(const Attn8Args& A, int64_t u, int lane) {
   Counts8 c = {0, 0};
-  for (int64_t u0 = 0; u0 < A.units; u0 += 64) {
+  for (int64_t u0 = 0; u0 < A.C.B; u0 += 64) {
     const int64_t v = u0 + lane;
-    const uint32_t n = v < A.units ? (uint32_t)unit8(A, v).tiles() : 0u;
+    const uint32_t n = v < A.C.B ? (uint32_t)unit_a(A, v).tiles() : 0u;
     c.all += wave_total(n);
     if (u0 < u) c.before += wave_total(v < u ? n : 0u);
   }
@@ -507,11 +585,6 @@ __device__ __forceinline__ Counts8 count8(const Attn8Args& A, int64_t u, int lan
 
 __device__ __forceinline__ int64_t group_share(const Attn8Args& A, int64_t all) {
   return max((all * A.C.KVH + A.groups - 1) / A.groups, (int64_t)kWavesA);
-}
-
-// Where a token of a tile stands against a row's position.
-__device__ __forceinline__ bool sees(int p, int pos, int window, int sink) {
-  return p <= pos && (window <= 0 || p < sink || p > pos - window);
 }
 
 // A wave's running softmax: lane (n, g) has row n; O[cb][r] is channel
@@ -540,11 +613,11 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
   const int64_t end = min(cur + share, all * C.KVH);
   if (cur >= end) return;
 
-  // the unit of tile `cur`
+  // the sequence of tile `cur`
   int64_t u = 0, base = 0;   // base: tiles of all heads before unit u
-  for (int64_t u0 = 0; u0 < A.units; u0 += 64) {
+  for (int64_t u0 = 0; u0 < C.B; u0 += 64) {
     const int64_t v = u0 + lane;
-    const uint32_t n = v < A.units ? (uint32_t)unit8(A, v).tiles() : 0u;
+    const uint32_t n = v < C.B ? (uint32_t)unit_a(A, v).tiles() : 0u;
     uint32_t upto = n;       // inclusive prefix
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -562,7 +635,7 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
   }
 
   while (cur < end) {
-    const Unit8 U = unit8(A, u);
+    const Unit8 U = unit_a(A, u);
     const int nt = U.tiles();
     if (nt == 0) {
       ++u;
@@ -609,40 +682,20 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
     for (int i0 = 0; i0 < own; i0 += 32) {
       const int n = min(own - i0, 32);
       // lane 2i + h: half h of the wave's tile i: its page, scales
-      int page = -1;
-      float kf = 0.f, lv = 0.f, inv = 1.f;
-      {
-        const int i = lane >> 1;
-        const int tok = kTile * U.tile(j0 + wave + kWavesA * (i0 + min(i, n - 1))) + 16 * (lane & 1);
-        if (i < n && tok < hi) {
-          const int id = C.bt[(int64_t)U.s.b * C.max_blocks + (tok >> C.ps_log2)];
-          if (id >= 0 && id < C.num_pages) {
-            page = id;
-            const int64_t at = scale_index(C, id, head, tok);
-            kf = C.ks[at] * A.scale_log2;
-            const float vs = C.vs[at];
-            // a scale that is hardly one counts as the writer's least
-            const float s = vs < 0x1p-100f ? 0x1p-100f : vs;
-            lv = __builtin_amdgcn_logf(s);
-            inv = s == s ? 1.f / s : 1.f;   // a NaN arrives through lv, where masks hold
-          }
-        }
-      }
+      const int mi = lane >> 1;
+      const int mtok = kTile * U.tile(j0 + wave + kWavesA * (i0 + min(mi, n - 1))) + 16 * (lane & 1);
+      const Meta8 meta = meta8(A, U.s.b, head, mtok, mi < n && mtok < hi);
       auto lane_f = [](float x, int l) {
         return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
       };
       auto tok_of = [&](int i) { return kTile * U.tile(j0 + wave + kWavesA * (i0 + i)); };
-      // every token of the tile is seen by every row
-      auto is_full = [&](int tok) {
-        return tok + kTile - 1 <= U.pos0 && (A.window <= 0 || tok + kTile <= sink || tok > U.pos1 - A.window);
-      };
       auto load = [&](int i, Raw8& X) {
         const bool live = i < n;
         const int tok = tok_of(live ? i : 0);
-        const bool full = is_full(tok);
+        const bool full = all_seen(A, U, tok, kTile);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int id = live ? __builtin_amdgcn_readlane(page, 2 * i + h) : -1;
+          const int id = live ? __builtin_amdgcn_readlane(meta.page, 2 * i + h) : -1;
           const uint32_t bytes = id >= 0 ? 15u * C.row_bytes + kCodeRow : 0u;
           const int64_t off = id >= 0 ? row_offset(C, id, 0, tok + 16 * h) : 0;
           const rsrc_t rk = make_rsrc(kbase + off, bytes), rv = make_rsrc(vbase + off, bytes);
@@ -660,7 +713,7 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
       };
       auto step = [&](int i, Raw8& X) {
         const int tok = tok_of(i);
-        const bool full = is_full(tok);
+        const bool full = all_seen(A, U, tok, kTile);
         // staged: K rows' 16-byte chunks turned by the row, V's by its place
         // among the eight rows that a transposed read takes
         const int r8 = lane >> 3, ch = lane & 7;
@@ -691,9 +744,9 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
           s1 = mfma16x16x32<E>(widen8<CODE, E>(u32x2{b[0], b[1]}), qB[2 * h2], s1);
           s1 = mfma16x16x32<E>(widen8<CODE, E>(u32x2{b[2], b[3]}), qB[2 * h2 + 1], s1);
         }
-        const float kf0 = lane_f(kf, 2 * i), kf1 = lane_f(kf, 2 * i + 1);
-        const float lv0 = lane_f(lv, 2 * i), lv1 = lane_f(lv, 2 * i + 1);
-        const float inv0 = lane_f(inv, 2 * i), inv1 = lane_f(inv, 2 * i + 1);
+        const float kf0 = lane_f(meta.kf, 2 * i), kf1 = lane_f(meta.kf, 2 * i + 1);
+        const float lv0 = lane_f(meta.lv, 2 * i), lv1 = lane_f(meta.lv, 2 * i + 1);
+        const float inv0 = lane_f(meta.inv, 2 * i), inv1 = lane_f(meta.inv, 2 * i + 1);
         float x[8];
         uint32_t seen = 0;
 #pragma unroll
@@ -792,10 +845,7 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
           acc += *reinterpret_cast<const float4v*>(lds + w * kSlotA + row * (kHeadDim * 4) + ((chunk ^ row) << 4)) * f[w];
         if (row < U.rows) {
           if (whole) {
-            const float d = L == 0.f ? 1.f : L;
-            const int r = U.row0 + row, tok = r / A.G;
-            uint16_t* out = (uint16_t*)A.o + ((int64_t)(U.s.c0 + tok) * A.H + head * A.G + (r - tok * A.G)) * kHeadDim + 4 * chunk;
-            *reinterpret_cast<u32x2*>(out) = round_elt4<E>(float4v{acc[0] / d, acc[1] / d, acc[2] / d, acc[3] / d});
+            store_out<E>(A, out_row(A, U, head, row) + 4 * chunk, acc, L);
           } else {
             *reinterpret_cast<float4v*>(A.part + (place * kRowsA + row) * kHeadDim + 4 * chunk) = acc;
           }
@@ -821,13 +871,12 @@ __global__ __launch_bounds__(256) void join8_kernel(Attn8Args A) {
   const int row = (int)(id % kRowsA);
   const int64_t pair = id / kRowsA, u = pair / C.KVH;
   const int head = (int)(pair - u * C.KVH);
-  const Unit8 U = unit8(A, u);
+  const Unit8 U = unit_a(A, u);
   if (row >= U.rows) return;
-  const int r = U.row0 + row, tok = r / A.G;
-  uint16_t* out = (uint16_t*)A.o + ((int64_t)(U.s.c0 + tok) * A.H + head * A.G + (r - tok * A.G)) * kHeadDim;
+  const int64_t out = out_row(A, U, head, row);
   const int nt = U.tiles();
   if (nt == 0) {
-    if (threadIdx.x < 32) *reinterpret_cast<u32x2*>(out + 4 * threadIdx.x) = u32x2{0u, 0u};
+    if (threadIdx.x < 32) store_out<E>(A, out + 4 * threadIdx.x, float4v{0.f, 0.f, 0.f, 0.f}, 0.f);
     return;
   }
   const Counts8 c = count8(A, u, lane);
@@ -860,8 +909,329 @@ __global__ __launch_bounds__(256) void join8_kernel(Attn8Args A) {
     acc += parts[w][chunk];
     L += sums[w];
   }
-  const float d = L == 0.f ? 1.f : L;
-  *reinterpret_cast<u32x2*>(out + 4 * chunk) = round_elt4<E>(float4v{acc[0] / d, acc[1] / d, acc[2] / d, acc[3] / d});
+  store_out<E>(A, out + 4 * chunk, acc, L);
+}
+
+// ---- the wide kernel ----
+//
+// One workgroup a pair (unit, KV head) and split: four waves of 32 query rows
+// each share a tile of 64 tokens, widened to fp16 (K: the query's type) in LDS
+// once for all, two tiles in turn.  K's rows are staged with their 16-byte
+// chunks turned by the row, V's with their 64-byte quarters turned by it, so
+// that neither the operand reads nor V's transposed ones collide in a bank.
+// The products are v_mfma_f32_32x32x16: S = K Q^T leaves lane (n, hf) row n's
+// tokens 8 (r / 4) + 4 hf + r % 4, which is the order that the transposed
+// reads give V^T's operand in.
+// Weights are rounded to fp16 once here (2^-11 of each, as the output itself
+// in fp16): a second product for the remainder would cost half as much again
+// of the kernel's bound.
+
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+
+template <int E>
+__device__ __forceinline__ float16v mfma32x32x16(u32x4 a, u32x4 b, float16v c) {
+  if constexpr (E == kEltBf16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(a), as_h8(b), c, 0, 0, 0);
+}
+
+// Transposed LDS read (ds_read_b64_tr_b16): in each group of 16 lanes, lane
+// 4j + h supplies row j's columns 4h .. 4h + 3 and lane i receives column i.
+__device__ __forceinline__ u32x2 lds_read_tr16(const char* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(p)));
+}
+
+// The two halves' values of a row (lanes n and n + 32) joined.
+__device__ __forceinline__ float half_max(float x) {
+  const uint32_t a = __builtin_bit_cast(uint32_t, x);
+  const auto s = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)s[0]), __builtin_bit_cast(float, (uint32_t)s[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const uint32_t a = __builtin_bit_cast(uint32_t, x);
+  const auto s = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  return __builtin_bit_cast(float, (uint32_t)s[0]) + __builtin_bit_cast(float, (uint32_t)s[1]);
+}
+
+constexpr int kRowB = 2 * kHeadDim;                 // bytes of a widened row
+constexpr int kTileBytesB = kTileB * kRowB;         // of K or of V
+constexpr int kChunkB = 64;                         // tiles whose Meta8 are held at once
+constexpr int kSegs = kTileB / 16;                  // 16-token segments of a tile
+static_assert(kChunkB * kSegs == kThreadsB, "a thread a segment");
+
+// The tiles of split s of a pair.
+__device__ __forceinline__ void split_tiles(const Attn8Args& A, int nt, int s, int& j0, int& j1) {
+  const int per = max((nt + A.splits - 1) / A.splits, 4);
+  j0 = min(s * per, nt);
+  j1 = min(j0 + per, nt);
+}
+
+template <int CODE, int E>
+__global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
+  __shared__ __align__(16) char ks[2][kTileBytesB], vs[2][kTileBytesB];
+  __shared__ Meta8 metas[kThreadsB];
+  // e4m3, tiles that not every row sees whole: whether V tile i & 3 has a NaN,
+  // and which channels of each token
+  __shared__ int nan_seen[4];
+  __shared__ __align__(16) uint8_t nan_map[2][kTileB][kHeadDim / 8];
+  const Cache8& C = A.C;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, hf = lane >> 5;
+  // KV heads fastest (they go to different XCDs' caches), then splits; the last
+  // rows of a sequence, which have the most tiles, first
+  uint32_t id = blockIdx.x;
+  const int head = (int)(id % (uint32_t)C.KVH);
+  id /= (uint32_t)C.KVH;
+  const int split = (int)(id % (uint32_t)A.splits);
+  const int64_t u = A.units - 1 - (int64_t)(id / (uint32_t)A.splits);
+  const Unit8 U = unit_b(A, u);
+  if (U.rows == 0) return;
+  const int nt = U.tiles();
+  int j0, j1;
+  split_tiles(A, nt, split, j0, j1);
+  const bool whole = j1 - j0 == nt;
+  if (j0 == j1 && !(whole && split == 0)) return;
+
+  const int my_row = 32 * wave + n;
+  const int my_tok = (U.row0 + my_row) / A.G, my_head = U.row0 + my_row - my_tok * A.G;
+  const bool mine = my_row < U.rows;
+  const int pos = mine ? U.s.len - U.s.n + my_tok : -1;
+  const bool busy = 32 * wave < U.rows;   // the wave has rows
+  u32x4 qB[8];
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    qB[s] = u32x4{0u, 0u, 0u, 0u};
+    if (mine)
+      qB[s] = *reinterpret_cast<const u32x4*>((const uint16_t*)A.q + (int64_t)(U.s.c0 + my_tok) * A.q_tok +
+                                              (int64_t)(head * A.G + my_head) * A.q_head + 16 * s + 8 * hf);
+  }
+  float16v O[4];
+#pragma unroll
+  for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) O[cb][r] = 0.f;
+  float m = -INFINITY, l = 0.f;   // no token seen yet; the lane's share of the sum
+
+  const int hi = U.pos1 + 1, lo = A.window > 0 ? max(U.pos0 - A.window + 1, 0) : 0;
+  const int sink = A.window > 0 ? A.sink : 0;
+  const char* kbase = C.k + head * C.head_bytes;
+  const char* vbase = C.v + head * C.head_bytes;
+  const int r4 = lane >> 4, ch = lane & 15;   // staging: row 16 i + 4 wave + r4, 8 codes from 8 ch
+
+  for (int i0 = j0; i0 < j1; i0 += kChunkB) {
+    const int cnt = min(j1 - i0, kChunkB);
+    __syncthreads();
+    {
+      const int i = threadIdx.x / kSegs;
+      const int tok = kTileB * U.tile(i0 + min(i, cnt - 1)) + 16 * (threadIdx.x % kSegs);
+      metas[threadIdx.x] = meta8(A, U.s.b, head, tok, i < cnt && tok < hi);
+      if (threadIdx.x < 4) nan_seen[threadIdx.x] = 0;
+    }
+    __syncthreads();
+
+    u32x2 kc[kSegs], vc[kSegs];   // codes on their way: of the tile after the next
+    auto load = [&](int i) {
+      const bool live = i < cnt;
+      const int tok = kTileB * U.tile(i0 + (live ? i : 0));
+      const bool full = all_seen(A, U, tok, kTileB);
+#pragma unroll
+      for (int g = 0; g < kSegs; ++g) {
+        const int page = live ? __builtin_amdgcn_readfirstlane(metas[kSegs * i + g].page) : -1;
+        const uint32_t bytes = page >= 0 ? 15u * C.row_bytes + kCodeRow : 0u;
+        const int64_t off = page >= 0 ? row_offset(C, page, 0, tok + 16 * g) : 0;
+        uint32_t o = (uint32_t)(4 * wave + r4) * C.row_bytes + 8u * ch;
+        if (!full) {   // rows that no query row sees read as zeros
+          const int p = tok + 16 * g + 4 * wave + r4;
+          if (!(p < hi && (p >= lo || p < sink))) o = kOOB;
+        }
+        typedef int v2i __attribute__((ext_vector_type(2)));
+        kc[g] = __builtin_bit_cast(u32x2, (v2i)__builtin_amdgcn_raw_buffer_load_b64(make_rsrc(kbase + off, bytes), o, 0, 0));
+        vc[g] = __builtin_bit_cast(u32x2, (v2i)__builtin_amdgcn_raw_buffer_load_b64(make_rsrc(vbase + off, bytes), o, 0, 0));
+      }
+    };
+    auto stage = [&](int i) {
+      const int buf = i & 1;
+      // a NaN of V must not meet the weight 0 of a row that does not see it: it
+      // is staged as 0 and noted
+      if (CODE == kE4m3 && i < cnt && !all_seen(A, U, kTileB * U.tile(i0 + i), kTileB)) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int g = 0; g < kSegs; ++g) {
+          uint32_t bits = 0;
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            const uint32_t bad = nan_codes(vc[g][d]) >> 7;   // 0 or 1 a byte
+            vc[g][d] &= ~(bad * 0xffu);
+            bits |= ((bad * 0x01020408u) >> 24) << (4 * d);
+          }
+          nan_map[buf][16 * g + 4 * wave + r4][ch] = (uint8_t)bits;
+          any |= bits;
+        }
+        if (__any(any != 0)) nan_seen[i & 3] = 1;
+      }
+#pragma unroll
+      for (int g = 0; g < kSegs; ++g) {
+        const int r = 16 * g + 4 * wave + r4;
+        *reinterpret_cast<u32x4*>(ks[buf] + r * kRowB + ((ch ^ (r & 15)) << 4)) = widen8<CODE, E>(kc[g]);
+        *reinterpret_cast<u32x4*>(vs[buf] + r * kRowB + ((ch ^ ((r & 3) << 2)) << 4)) = widen8<CODE, kEltF16>(vc[g]);
+      }
+    };
+
+    load(0);
+    stage(0);
+    load(1);
+    __syncthreads();
+    for (int i = 0; i < cnt; ++i) {
+      const int tok = kTileB * U.tile(i0 + i);
+      const bool full = all_seen(A, U, tok, kTileB);
+      const bool nans = CODE == kE4m3 && !full && nan_seen[i & 3];
+      if (CODE == kE4m3 && threadIdx.x == 0) nan_seen[(i + 2) & 3] = 0;
+      stage(i + 1);   // (past the last tile: zeros)
+      load(i + 2);
+      if (busy) {
+        float16v S[2];
+        const char* kt = ks[i & 1];
+        const char* vt = vs[i & 1];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) S[b][r] = 0.f;
+#pragma unroll
+          for (int s = 0; s < 8; ++s)
+            S[b] = mfma32x32x16<E>(*reinterpret_cast<const u32x4*>(kt + (32 * b + n) * kRowB + (((2 * s + hf) ^ (n & 15)) << 4)),
+                                   qB[s], S[b]);
+        }
+        // logits against the running maximum (0 while there is none)
+        const float ref = m == -INFINITY ? 0.f : m;
+        float inv[kSegs], top = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < kSegs; ++g) {
+          const Meta8 mt = metas[kSegs * i + g];
+          inv[g] = mt.inv;
+          const float add = mt.lv - ref;
+#pragma unroll
+          for (int r = 8 * (g & 1); r < 8 * (g & 1) + 8; ++r) {
+            float x = __builtin_fmaf(S[g >> 1][r], mt.kf, add);
+            if (!full) {
+              x = sees(tok + 32 * (g >> 1) + 8 * (r >> 2) + 4 * hf + (r & 3), pos, A.window, A.sink) ? x : -INFINITY;
+            }
+            top = fmaxf(top, x);
+            S[g >> 1][r] = x;
+          }
+        }
+        if (__any(top > (m == -INFINITY ? -INFINITY : kRescaleSlack))) {
+          const float t = half_max(top);
+          const float now = m == -INFINITY ? t : fmaxf(m, m + t);
+          const float to = now == -INFINITY ? 0.f : now;
+          const float f = __builtin_amdgcn_exp2f(m - to);   // 0 while there was none
+          const float d = ref - to;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[b][r] += d;
+          l *= f;
+#pragma unroll
+          for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) O[cb][r] *= f;
+          m = now;
+        }
+        u32x4 P[kSegs];
+#pragma unroll
+        for (int g = 0; g < kSegs; ++g) {
+          half8 h;
+          float sum = 0.f;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const float w = __builtin_amdgcn_exp2f(S[g >> 1][8 * (g & 1) + r]);
+            sum += w;
+            h[r] = (_Float16)w;
+          }
+          l = __builtin_fmaf(sum, inv[g], l);
+          P[g] = as_u4(h);
+        }
+        // lane (group of 16 lanes, 4j + h): row 4 hf + j, channel 16 (group & 1) + 4 h
+        const int j = (lane >> 2) & 3;
+        const char* vl = vt + (4 * hf + j) * kRowB + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+        auto values = [&](int g, int cb) {
+          const u32x2 a = lds_read_tr16(vl + 16 * g * kRowB + ((cb ^ j) << 6));
+          const u32x2 b = lds_read_tr16(vl + (16 * g + 8) * kRowB + ((cb ^ j) << 6));
+          return u32x4{a[0], a[1], b[0], b[1]};
+        };
+#pragma unroll
+        for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+          for (int g = 0; g < kSegs; ++g) O[cb] = mfma32x32x16<kEltF16>(values(g, cb), P[g], O[cb]);
+        if (nans) {   // and reaches the rows that do
+          u32x4 hit = {0u, 0u, 0u, 0u};   // this row's channels
+          for (int p = 0; p < kTileB; ++p)
+            if (sees(tok + p, pos, A.window, A.sink)) hit |= *reinterpret_cast<const u32x4*>(nan_map[i & 1][p]);
+#pragma unroll
+          for (int cb = 0; cb < 4; ++cb) {
+            const uint32_t w = hit[cb] >> (4 * hf);
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              O[cb][r] = w >> (8 * (r >> 2) + (r & 3)) & 1u ? __builtin_nanf("") : O[cb][r];
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+
+  if (!mine) return;
+  l = half_sum(l);
+  const int64_t at = whole ? out_row(A, U, head, my_row) : (((u * C.KVH + head) * A.splits + split) * kRowsB + my_row) * kHeadDim;
+#pragma unroll
+  for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int64_t c = at + 32 * cb + 2 * r + 4 * hf;
+      const float4v v = {O[cb][r], O[cb][r + 1], O[cb][r + 2], O[cb][r + 3]};
+      if (whole)
+        store_out<E>(A, c, v, l);
+      else
+        *reinterpret_cast<float4v*>(A.part + c) = v;
+    }
+  if (!whole && hf == 0) {
+    float* ml = A.part + A.units * C.KVH * A.splits * kRowsB * kHeadDim;
+    ml[at / kHeadDim] = m;
+    ml[A.units * C.KVH * A.splits * kRowsB + at / kHeadDim] = l;
+  }
+}
+
+// Joins the splits of the wide kernel's rows, 32 threads a row.
+template <int E>
+__global__ __launch_bounds__(256) void wide_join8_kernel(Attn8Args A) {
+  const Cache8& C = A.C;
+  const int64_t pair = blockIdx.x / (kRowsB / 8);
+  const int row = 8 * (int)(blockIdx.x % (kRowsB / 8)) + (threadIdx.x >> 5), chunk = threadIdx.x & 31;
+  const int64_t u = pair / C.KVH;
+  const int head = (int)(pair - u * C.KVH);
+  const Unit8 U = unit_b(A, u);
+  const int nt = U.tiles();
+  int j0, j1;
+  split_tiles(A, nt, 0, j0, j1);
+  if (row >= U.rows || j1 == nt) return;
+  const int64_t rows = A.units * C.KVH * A.splits * kRowsB;
+  const float* pm = A.part + rows * kHeadDim;
+  const float* pl = pm + rows;
+  const int64_t first = pair * A.splits * kRowsB + row;
+  const int splits = (nt + j1 - 1) / j1;
+  float M = -INFINITY;
+  for (int s = 0; s < splits; ++s) M = fmaxf(M, pm[first + s * kRowsB]);
+  const float ref = M == -INFINITY ? 0.f : M;
+  float4v acc = {0.f, 0.f, 0.f, 0.f};
+  float L = 0.f;
+  for (int s = 0; s < splits; ++s) {
+    const int64_t p = first + s * kRowsB;
+    const float f = __builtin_amdgcn_exp2f(pm[p] - ref);
+    L = __builtin_fmaf(pl[p], f, L);
+    acc += *reinterpret_cast<const float4v*>(A.part + p * kHeadDim + 4 * chunk) * f;
+  }
+  store_out<E>(A, out_row(A, U, head, row) + 4 * chunk, acc, L);
 }
 
 // ---------------------------------------------------------------------------
@@ -951,23 +1321,49 @@ int launch_read(const Read8Args& A, int dtype, hipStream_t stream) {
   return launch_status();
 }
 
-// Units of a call (with those of the rows past the last sequence), and its
-// workgroups: no more than there can be runs of one tile a wave.
-int64_t attn_units(bool offsets, int64_t B, int64_t T, int64_t G) {
-  return offsets ? T * G / kRowsA + B + 1 : B * ((G + kRowsA - 1) / kRowsA);
-}
-int attn_groups(int64_t units, int32_t KVH, int64_t max_len) {
-  const int64_t tiles = units * KVH * ((max_len + kTile - 1) / kTile);
+// Narrow kernel: workgroups, no more than there can be runs of one tile a wave;
+// none if no sequence can have so few rows.
+int narrow_groups(bool offsets, int64_t B, int32_t KVH, int32_t G, int64_t max_len) {
+  if (G > kRowsA) return 0;
+  const int64_t tiles = B * KVH * ((max_len + kTile - 1) / kTile);
   return (int)std::min<int64_t>(kGroupsA, std::max<int64_t>(1, (tiles + kWavesA - 1) / kWavesA));
 }
-size_t part_bytes(int groups) { return (size_t)2 * groups * kRowsA * (kHeadDim + 2) * sizeof(float); }
+size_t narrow_bytes(int groups) { return (size_t)2 * groups * kRowsA * (kHeadDim + 2) * sizeof(float); }
+
+// Wide kernel: units of a call (with those of the rows past the last sequence),
+// and splits a pair where the pairs do not fill the GPU.
+int64_t wide_units(bool offsets, int64_t B, int64_t T, int32_t G) {
+  if (!offsets) return G > kRowsA ? B * ((G + kRowsB - 1) / kRowsB) : 0;
+  return T * G / kRowsB + B + 1;
+}
+int wide_splits(int64_t units, int32_t KVH, int64_t max_len) {
+  const int64_t pairs = std::max<int64_t>(units * KVH, 1), tiles = (max_len + kTileB - 1) / kTileB;
+  return (int)std::max<int64_t>(1, std::min((kPairsB + pairs - 1) / pairs, tiles / 4));
+}
+size_t wide_bytes(int64_t units, int32_t KVH, int splits) {
+  return splits <= 1 ? 0 : (size_t)units * KVH * splits * kRowsB * (kHeadDim + 2) * sizeof(float);
+}
+
+size_t attn_bytes(bool offsets, int64_t B, int64_t T, int32_t G, int32_t KVH, int64_t max_len) {
+  const int64_t units = wide_units(offsets, B, T, G);
+  return std::max(narrow_bytes(narrow_groups(offsets, B, KVH, G, max_len)),
+                  wide_bytes(units, KVH, wide_splits(units, KVH, max_len)));
+}
 
 template <int CODE, int E>
-int launch_attn8(const Attn8Args& A, hipStream_t stream) {
-  attn8_kernel<CODE, E><<<dim3((unsigned)A.groups), dim3(kThreadsA), 0, stream>>>(A);
-  const int rc = launch_status();
-  if (rc) return rc;
-  join8_kernel<E><<<dim3((unsigned)(A.units * A.C.KVH * kRowsA)), dim3(256), 0, stream>>>(A);
+int launch_attn8(Attn8Args A, hipStream_t stream) {
+  // one after the other: both kernels' partial rows go to the same workspace
+  if (A.groups > 0) {
+    attn8_kernel<CODE, E><<<dim3((unsigned)A.groups), dim3(kThreadsA), 0, stream>>>(A);
+    join8_kernel<E><<<dim3((unsigned)(A.C.B * A.C.KVH * kRowsA)), dim3(256), 0, stream>>>(A);
+    const int rc = launch_status();
+    if (rc) return rc;
+  }
+  if (A.units > 0) {
+    wide8_kernel<CODE, E><<<dim3((unsigned)(A.units * A.C.KVH * A.splits)), dim3(kThreadsB), 0, stream>>>(A);
+    if (A.splits > 1)
+      wide_join8_kernel<E><<<dim3((unsigned)(A.units * A.C.KVH * (kRowsB / 8))), dim3(256), 0, stream>>>(A);
+  }
   return launch_status();
 }
 
@@ -1017,7 +1413,7 @@ int kvdec_paged8_read(const kvdec_paged8_cache* cache, const int32_t* cu_seqlens
 size_t kvdec_paged8_workspace_bytes(int64_t B, int64_t T, int32_t H, int32_t KVH, int64_t max_len) {
   if (B < 1 || T < 1 || H < 1 || KVH < 1 || H % KVH || max_len < 1 || max_len >= ((int64_t)1 << 30)) return 0;
   if (B >= ((int64_t)1 << 24) || T * (H / KVH) >= ((int64_t)1 << 30)) return 0;
-  return part_bytes(attn_groups(attn_units(true, B, T, H / KVH), KVH, max_len));
+  return std::max(attn_bytes(true, B, T, H / KVH, KVH, max_len), T == B ? attn_bytes(false, B, T, H / KVH, KVH, max_len) : 0);
 }
 
 int kvdec_paged8_attention(const kvdec_paged8_cache* cache, const void* q, void* o, int dtype,
@@ -1034,10 +1430,13 @@ int kvdec_paged8_attention(const kvdec_paged8_cache* cache, const void* q, void*
   if (T * A.G >= ((int64_t)1 << 30)) return KVDEC_E_SHAPE;
   if (window < 0 || sink < 0 || (window == 0 && sink > 0)) return KVDEC_E_WINDOW;
   if (!on16(q) || !on16(o) || q_token_stride % 8 || q_head_stride % 8) return KVDEC_E_UNSUPPORTED;
-  A.units = attn_units(cu_seqlens != nullptr, B, T, A.G);
-  if (A.units * A.C.KVH * kRowsA > 0x7fffffff) return KVDEC_E_SHAPE;
-  A.groups = attn_groups(attn_units(true, B, T, A.G), A.C.KVH, A.C.max_len);
-  if (!ws || !on16(ws) || ws_bytes < part_bytes(A.groups)) return KVDEC_E_WORKSPACE;
+  const bool offsets = cu_seqlens != nullptr;
+  A.groups = narrow_groups(offsets, B, A.C.KVH, A.G, A.C.max_len);
+  A.units = wide_units(offsets, B, T, A.G);
+  A.splits = wide_splits(A.units, A.C.KVH, A.C.max_len);
+  if (B * A.C.KVH * kRowsA > 0x7fffffff || A.units * A.C.KVH * std::max(A.splits, kRowsB / 8) > 0x7fffffff)
+    return KVDEC_E_SHAPE;
+  if (!ws || !on16(ws) || ws_bytes < attn_bytes(offsets, B, T, A.G, A.C.KVH, A.C.max_len)) return KVDEC_E_WORKSPACE;
   A.q = q;
   A.o = o;
   A.part = static_cast<float*>(ws);

@@ -179,8 +179,10 @@ def test_workspace_bytes():
     f = K.lib.kvdec_paged8_workspace_bytes
     assert f(0, 1, 64, 8, 100) == 0 == f(1, 0, 64, 8, 100) == f(1, 1, 60, 8, 100) == f(1, 1, 64, 8, 0)
     assert f(1, 1, 64, 8, 1 << 30) == 0
-    most = f(1 << 20, 1 << 20, 64, 8, (1 << 30) - 1)
-    assert 0 < f(1, 1, 8, 8, 16) <= f(32, 32, 64, 8, 163840) <= most < 1 << 28
+    # bounded whatever the batch, the new tokens and the lengths
+    for B, T, H, KVH, n in ((1, 1, 8, 8, 16), (32, 32, 64, 8, 163840), (1, 2048, 64, 8, 8192), (8, 40, 64, 8, 4096),
+                            (1, 1, 64, 1, 1 << 20), (1 << 20, 1 << 20, 64, 8, (1 << 30) - 1)):
+        assert 0 < f(B, T, H, KVH, n) < 1 << 28
 
 
 def test_wrappers_refuse():
