@@ -62,18 +62,42 @@ __device__ __forceinline__ Seq8 seq8(const Cache8& C, int64_t b) {
   return s;
 }
 
-// Units of work without a count on the host: sequence b starts at a unit
-// first(b) that grows with the rows before it by what a unit holds, and by as
-// many more a sequence as its rows can touch beyond that.  The sequence of unit
-// u is the last with first(b) <= u; first(0) is 0.
+// Units of work without a count on the host: sequence b, whose first new token
+// is c0, starts at unit first(c0, b), which grows with the rows before it by what
+// a unit holds, and by as many more a sequence as its rows can touch beyond that;
+// first(0, 0) is 0.  The sequence of unit u is the last with first <= u: 64 are
+// tried at once, a lane each, so that a search among 64 is one load's latency.
+struct Found8 {
+  Seq8 s;
+  int64_t first;
+};
 template <class First>
-__device__ __forceinline__ int64_t seq_of_unit(int64_t B, int64_t u, First&& first) {
-  int64_t lo = 0, hi = B;   // B: the rows past the last sequence
-  while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) >> 1;
-    if (first(mid) <= u) lo = mid; else hi = mid - 1;
+__device__ __forceinline__ Found8 find8(const Cache8& C, int64_t u, int lane, First&& first) {
+  int64_t lo = 0, n = C.B + 1;   // B: the rows past the last sequence
+  while (n > 64) {
+    const int64_t step = (n + 63) / 64, s = lo + lane * step;
+    const bool ok = s < lo + n && first(offset8(C, s), s) <= u;
+    const int cnt = max((int)__builtin_popcountll(__ballot(ok)), 1);
+    const int64_t to = lo + (cnt - 1) * step;
+    n = min(step, lo + n - to);
+    lo = to;
   }
-  return lo;
+  const int64_t s = lo + lane;
+  int c0 = 0, c1 = 0, len = 0;
+  if (lane < n) {
+    c0 = offset8(C, s);
+    c1 = s < C.B ? offset8(C, s + 1) : (int)C.T;
+    if (s < C.B) len = min(max(((const int32_t*)C.lens)[s], 0), C.max_len);
+  }
+  const bool ok = lane < n && first(c0, s) <= u;
+  const int at = __builtin_amdgcn_readfirstlane(max((int)__builtin_popcountll(__ballot(ok)), 1) - 1);
+  Found8 f;
+  f.s.b = __builtin_amdgcn_readfirstlane((int)lo) + at;
+  f.s.c0 = __builtin_amdgcn_readlane(c0, at);
+  f.s.n = __builtin_amdgcn_readlane(c1, at) - f.s.c0;
+  f.s.len = __builtin_amdgcn_readlane(len, at);
+  f.first = first(f.s.c0, (int64_t)f.s.b);
+  return f;
 }
 
 // The tokens of unit u that lie in one block of one sequence: rows [r0, r1) of
@@ -85,17 +109,16 @@ struct Run8 {
   int64_t page;
 };
 
-__device__ __forceinline__ Run8 run8(const Cache8& C, int64_t u) {
-  int64_t b, j;
+__device__ __forceinline__ Run8 run8(const Cache8& C, int64_t u, int lane) {
+  Seq8 s;
+  int64_t j = 0;
   if (C.cu == nullptr) {
-    b = u;
-    j = 0;
+    s = seq8(C, u);
   } else {
-    auto first = [&](int64_t s) { return ((int64_t)offset8(C, s) >> C.blk_log2) + 2 * s; };
-    b = seq_of_unit(C.B, u, first);
-    j = u - first(b);
+    const Found8 f = find8(C, u, lane, [&](int c0, int64_t b) { return ((int64_t)c0 >> C.blk_log2) + 2 * b; });
+    s = f.s;
+    j = u - f.first;
   }
-  const Seq8 s = seq8(C, b);
   const int64_t p0 = (int64_t)s.len - s.n, block = (int64_t)1 << C.blk_log2;
   Run8 r;
   r.start = ((p0 >> C.blk_log2) + j) << C.blk_log2;
@@ -104,7 +127,7 @@ __device__ __forceinline__ Run8 run8(const Cache8& C, int64_t u) {
   r.r1 = s.n > 0 ? (int)max(min((int64_t)s.len - r.start, block), (int64_t)0) : 0;
   r.page = -1;
   if (r.r1 > r.r0 && r.start >= 0) {   // then start < len <= max_len
-    const int64_t id = ((cint32*)C.bt)[b * C.max_blocks + (r.start >> C.ps_log2)];
+    const int64_t id = ((cint32*)C.bt)[(int64_t)s.b * C.max_blocks + (r.start >> C.ps_log2)];
     if (id >= 0 && id < C.num_pages) r.page = id;
   }
   return r;
@@ -168,31 +191,28 @@ __device__ __forceinline__ float4v code_values(uint32_t c) {
   }
 }
 
-__device__ __forceinline__ bool finite32(float x) { return __builtin_fabsf(x) <= 3.402823466e38f; }
-
-// Four values in the codes' range, rounded to codes (ties to even).  e4m3:
-// anything not finite becomes the NaN code.
-template <int CODE>
-__device__ __forceinline__ uint32_t to_codes(float4v x) {
-  if constexpr (CODE == kE4m3) {
-    int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-    c = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], c, true);
-    uint32_t r = (uint32_t)c;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (!finite32(x[j])) r = (r & ~(0xffu << (8 * j))) | (0x7fu << (8 * j));
-    return r;
-  } else {
-    uint32_t r = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r |= ((uint32_t)(int)__builtin_rintf(x[j]) & 0xffu) << (8 * j);
-    return r;
-  }
-}
-
 // The high bit of every byte of c that is a NaN of e4m3.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t c) {
   return ((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+// Four values x * m in the codes' range, rounded to codes, ties to even, in one
+// rounding where x * m is exact (m a power of two).  e4m3: a NaN is the code
+// 0x7f.  int8: added to 1.5 * 2^23, whose last bits are units, it is rounded to
+// the byte that the sum ends in.
+template <int CODE>
+__device__ __forceinline__ uint32_t to_codes(float4v x, float m) {
+  if constexpr (CODE == kE4m3) {
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * m, x[1] * m, 0, false);
+    c = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * m, x[3] * m, c, true);
+    return (uint32_t)c & ~nan_codes((uint32_t)c);
+  } else {
+    uint32_t b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = __builtin_bit_cast(uint32_t, __builtin_fmaf(x[j], m, 12582912.f));
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u),
+                                 __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), 0x05040100u);
+  }
 }
 
 // The least power of two s >= 2^kLowest with amax <= s * (448 or 127).
@@ -217,28 +237,51 @@ struct Write8Args {
   int64_t tasks;                          // units * 2 * KVH
 };
 
-// Eight elements of a row as floats.
+constexpr float kFloatMax = 3.402823466e38f;
+
+// Eight elements of a row as they are loaded.  The largest |element| of several
+// is kept as bits (of all NaN and infinities above the rest): `Top` in the
+// loaded form, and then as those of a float.
 template <class T>
-__device__ __forceinline__ void load_row8(const T* p, float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4v a = *reinterpret_cast<const float4v*>(p), b = *reinterpret_cast<const float4v*>(p + 4);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[j] = a[j];
-      x[4 + j] = b[j];
-    }
-  } else {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint16_t h = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
-      if constexpr (std::is_same<T, _Float16>::value)
-        x[j] = (float)__builtin_bit_cast(_Float16, h);
-      else
-        x[j] = __builtin_bit_cast(float, (uint32_t)h << 16);
-    }
+struct Row8 {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  typedef u16x2 Top;
+  u32x4 w = {0u, 0u, 0u, 0u};
+  __device__ __forceinline__ void load(const T* p) { w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)); }
+  __device__ __forceinline__ float get(int j) const {
+    const uint16_t h = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+    if constexpr (std::is_same<T, _Float16>::value)
+      return (float)__builtin_bit_cast(_Float16, h);
+    else
+      return __builtin_bit_cast(float, (uint32_t)h << 16);
   }
-}
+  __device__ __forceinline__ void top(Top& m) const {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[d] & 0x7fff7fffu));
+  }
+  __device__ static __forceinline__ uint32_t bits(Top m) {
+    const uint16_t h = m[0] > m[1] ? m[0] : m[1];
+    if constexpr (std::is_same<T, _Float16>::value)
+      return h >= 0x7c00 ? 0x7f800000u : __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(_Float16, h));
+    else
+      return (uint32_t)h << 16;
+  }
+};
+template <>
+struct Row8<float> {
+  typedef uint32_t Top;
+  u32x4 w[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
+  __device__ __forceinline__ void load(const float* p) {
+    w[0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+    w[1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 4));
+  }
+  __device__ __forceinline__ float get(int j) const { return __builtin_bit_cast(float, (uint32_t)w[j >> 2][j & 3]); }
+  __device__ __forceinline__ void top(Top& m) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, w[j >> 2][j & 3] & 0x7fffffffu);
+  }
+  __device__ static __forceinline__ uint32_t bits(Top m) { return m; }
+};
 
 constexpr int kWriteWaves = 4;
 
@@ -262,40 +305,47 @@ __global__ __launch_bounds__(64 * kWriteWaves) void write8_kernel(Write8Args A) 
     const int64_t rest = task / C.KVH;
     head = (int)(task - rest * C.KVH);
     kv = (int)(rest & 1);
-    run = run8(C, rest >> 1);
+    run = run8(C, rest >> 1, lane);
   }
   const bool live = run.page >= 0;   // (uniform over a task's waves)
   const int base = part * kRows;
 
-  float x[kLoads][8];
-  float amax = 0.f;
-  bool bad = false;
+  Row8<T> x[kLoads];
+  uint32_t top = 0;      // the largest |x|: the bits of a float
   float old = 0.f;
   float* scale = nullptr;
   char* codes = nullptr;
   if (live) {
     scale = (kv ? C.vs : C.ks) + scale_index(C, run.page, head, run.start);
     codes = (kv ? C.v : C.k) + row_offset(C, run.page, head, run.start);
-    if (run.r0 > 0) old = *scale;
     const T* src = (const T*)A.x[kv] + run.c * A.tok_stride[kv] + head * A.head_stride[kv] + 8 * t;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int r = base + 4 * i + g;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[i][j] = 0.f;
-      if (r >= run.r0 && r < run.r1) load_row8(src + r * A.tok_stride[kv], x[i]);
+      if (r >= run.r0 && r < run.r1) x[i].load(src + r * A.tok_stride[kv]);
     }
+    if (run.r0 > 0) old = *scale;
+    typename Row8<T>::Top m{};
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) x[i].top(m);
+    top = Row8<T>::bits(m);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
+    top = (uint32_t)__builtin_amdgcn_readfirstlane((int)top);
+  }
+  bool bad = top >= 0x7f800000u;
+  float amax = __builtin_bit_cast(float, top);
+  if (bad) {   // once more, of the finite ones
+    amax = 0.f;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const bool ok = finite32(x[i][j]);
-        bad = bad || !ok;
-        amax = ok ? fmaxf(amax, __builtin_fabsf(x[i][j])) : amax;
+        const float a = __builtin_fabsf(x[i].get(j));
+        amax = a <= kFloatMax ? fmaxf(amax, a) : amax;
       }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
-    bad = __any(bad);
   }
   if constexpr (kPer > 1) {
     __shared__ float wave_max[kWriteWaves];
@@ -330,30 +380,34 @@ __global__ __launch_bounds__(64 * kWriteWaves) void write8_kernel(Write8Args A) 
       u32x4* p = reinterpret_cast<u32x4*>(codes + (int64_t)r * C.row_bytes + col);
       u32x4 c = *p;
 #pragma unroll
-      for (int d = 0; d < 4; ++d) c[d] = to_codes<CODE>(code_values<CODE>(c[d]) * ratio);
+      for (int d = 0; d < 4; ++d) c[d] = to_codes<CODE>(code_values<CODE>(c[d]), ratio);
       *p = c;
     }
   }
 
+  auto store = [&](auto&& value, float m) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = base + 4 * i + g;
+      u32x2 c;
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        float4v y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = value(x[i].get(4 * d + j));
+        c[d] = poison ? 0u : to_codes<CODE>(y, m);
+      }
+      if (r >= run.r0 && r < run.r1) *reinterpret_cast<u32x2*>(codes + (int64_t)r * C.row_bytes + 8 * t) = c;
+    }
+  };
   // A power of two divides by its inverse, exactly; a scale that some other
   // program put there may be any.
-  const uint32_t sb = __builtin_bit_cast(uint32_t, s);
+  const uint32_t sb = (uint32_t)__builtin_amdgcn_readfirstlane((int)__builtin_bit_cast(uint32_t, s));
   const bool pow2 = (sb & 0x7fffffu) == 0 && sb < 0x7f000000u;
-  const float inv = __builtin_bit_cast(float, 0x7f000000u - sb);
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int r = base + 4 * i + g;
-    if (r < run.r0 || r >= run.r1) continue;
-    u32x2 c;
-#pragma unroll
-    for (int d = 0; d < 2; ++d) {
-      float4v y;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = pow2 ? x[i][4 * d + j] * inv : x[i][4 * d + j] / s;
-      c[d] = poison ? 0u : to_codes<CODE>(y);
-    }
-    *reinterpret_cast<u32x2*>(codes + (int64_t)r * C.row_bytes + 8 * t) = c;
-  }
+  if (pow2 && !bad)
+    store([](float v) { return v; }, __builtin_bit_cast(float, 0x7f000000u - sb));
+  else
+    store([s](float v) { return __builtin_fabsf(v) <= kFloatMax ? v / s : __builtin_nanf(""); }, 1.f);
   if (part == 0 && lane == 0) *scale = s;
 }
 
@@ -367,16 +421,10 @@ struct Read8Args {
   int64_t tasks;
 };
 
-template <class T>
-__device__ __forceinline__ void store_values4(T* p, float4v v) {
-  if constexpr (sizeof(T) == 4)
-    *reinterpret_cast<float4v*>(p) = v;
-  else
-    *reinterpret_cast<u32x2*>(p) = round_elt4<std::is_same<T, _Float16>::value ? kEltF16 : kEltBf16>(v);
-}
-
-// One wave reads the call's rows of one block of one KV head, of K or of V,
-// eight rows an instruction.
+// One wave reads the call's rows of one block of one KV head, of K or of V: a
+// lane 8 codes of a row, four rows an instruction, so that 16-bit rows leave as
+// whole 256-byte ones.  The codes are read past the caches, which the rows
+// written need.
 template <int CODE, class T>
 __global__ __launch_bounds__(64 * kWriteWaves) void read8_kernel(Read8Args A) {
   const Cache8& C = A.C;
@@ -385,8 +433,8 @@ __global__ __launch_bounds__(64 * kWriteWaves) void read8_kernel(Read8Args A) {
   if (task >= A.tasks) return;
   const int64_t rest = task / C.KVH;
   const int head = (int)(task - rest * C.KVH), kv = (int)(rest & 1);
-  const Run8 run = run8(C, rest >> 1);
-  const int row8 = lane >> 3, col = 16 * (lane & 7);
+  const Run8 run = run8(C, rest >> 1, lane);
+  const int g = lane >> 4, col = 8 * (lane & 15);
   float scale = 0.f;
   const char* codes = nullptr;
   if (run.page >= 0) {
@@ -394,12 +442,30 @@ __global__ __launch_bounds__(64 * kWriteWaves) void read8_kernel(Read8Args A) {
     codes = (kv ? C.v : C.k) + row_offset(C, run.page, head, run.start) + col;
   }
   T* out = (T*)A.out[kv] + (run.c * C.KVH + head) * kHeadDim + col;
-  for (int r = run.r0 + row8; r < run.r1; r += 8) {
-    u32x4 c = {0u, 0u, 0u, 0u};
-    if (run.page >= 0) c = *reinterpret_cast<const u32x4*>(codes + (int64_t)r * C.row_bytes);
-    T* p = out + (int64_t)r * C.KVH * kHeadDim;
+  for (int r0 = run.r0; r0 < run.r1; r0 += 32) {   // eight loads on their way
+    u32x2 c[8];
 #pragma unroll
-    for (int d = 0; d < 4; ++d) store_values4(p + 4 * d, code_values<CODE>(c[d]) * scale);
+    for (int k = 0; k < 8; ++k) {
+      const int r = r0 + 4 * k + g;
+      c[k] = u32x2{0u, 0u};
+      if (run.page >= 0 && r < run.r1)
+        c[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(codes + (int64_t)r * C.row_bytes));
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int r = r0 + 4 * k + g;
+      if (r >= run.r1) continue;
+      T* p = out + (int64_t)r * C.KVH * kHeadDim;
+      const float4v lo = code_values<CODE>(c[k][0]) * scale, hi = code_values<CODE>(c[k][1]) * scale;
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4v*>(p) = lo;
+        *reinterpret_cast<float4v*>(p + 4) = hi;
+      } else {
+        constexpr int kElt = std::is_same<T, _Float16>::value ? kEltF16 : kEltBf16;
+        const u32x2 a = round_elt4<kElt>(lo), b = round_elt4<kElt>(hi);
+        *reinterpret_cast<u32x4*>(p) = u32x4{a[0], a[1], b[0], b[1]};
+      }
+    }
   }
 }
 
@@ -423,7 +489,7 @@ constexpr int kRowsA = 16;
 constexpr int kWavesA = 4;
 constexpr int kThreadsA = 64 * kWavesA;
 constexpr int kSlotA = 2 * kTile * kCodeRow;        // K and V codes of a tile
-constexpr int kGroupsA = 1024;                      // workgroups of a launch, at most
+constexpr int kGroupsA = 512;                       // workgroups of a launch, at most: two a CU
 static_assert(kRowsA * kHeadDim * 4 <= kSlotA, "a wave's partial rows fit its slot");
 
 constexpr int kRowsB = 128;                         // query rows of a workgroup, 32 a wave
@@ -439,7 +505,8 @@ struct Attn8Args {
   int64_t q_tok, q_head;      // in elements
   int64_t units;
   int32_t G, H, window, sink;
-  int32_t groups;             // narrow: workgroups
+  int32_t groups;             // narrow: workgroups,
+  int32_t side;               // and KV heads that one may read side by side (1, 2 or 4)
   int32_t splits;             // wide: workgroups a pair
   float scale_log2;
 };
@@ -483,37 +550,49 @@ __device__ __forceinline__ Unit8 unit_a(const Attn8Args& A, int64_t b) {
   return U;
 }
 
+// The same by halving, on scalars alone (the wide kernel has no registers for the
+// search above: 15% of its time).
+template <class First>
+__device__ __forceinline__ Found8 find8_scalar(const Cache8& C, int64_t u, First&& first) {
+  int64_t lo = 0, hi = C.B;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi + 1) >> 1;
+    if (first(offset8(C, mid), mid) <= u) lo = mid; else hi = mid - 1;
+  }
+  const Seq8 s = seq8(C, lo);
+  return Found8{s, first(s.c0, lo)};
+}
+
 // The wide kernel's unit u: kRowsB rows of a sequence of more than kRowsA, or of
 // the rows past the last sequence (which attend to nothing).
 __device__ __forceinline__ Unit8 unit_b(const Attn8Args& A, int64_t u) {
   const Cache8& C = A.C;
   Unit8 U;
-  int64_t b, first;
+  int64_t first;
   if (C.cu == nullptr) {
     const int per = (A.G + kRowsB - 1) / kRowsB;
-    b = u / per;
-    first = b * per;
+    first = u / per * per;
+    U.s = seq8(C, u / per);
   } else {
-    auto start = [&](int64_t s) { return (int64_t)offset8(C, s) * A.G / kRowsB + s; };
-    b = seq_of_unit(C.B, u, start);
-    first = start(b);
+    const Found8 f = find8_scalar(C, u, [&](int c0, int64_t b) { return (int64_t)c0 * A.G / kRowsB + b; });
+    U.s = f.s;
+    first = f.first;
   }
-  U.s = seq8(C, b);
-  const int64_t rows = (int64_t)U.s.n * A.G, row0 = (u - first) * kRowsB;
+  const int64_t rows = (int64_t)U.s.n * A.G, row0 = max(u - first, (int64_t)0) * kRowsB;
   U.row0 = (int)min(row0, rows);
-  U.rows = rows > kRowsA || b == C.B ? (int)min(rows - U.row0, (int64_t)kRowsB) : 0;
+  U.rows = rows > kRowsA || U.s.b == C.B ? (int)min(rows - U.row0, (int64_t)kRowsB) : 0;
   unit_tiles<kTileB>(A, U);
   return U;
 }
 
 // Where a token of a tile stands against a row's position.
 __device__ __forceinline__ bool sees(int p, int pos, int window, int sink) {
-  return p <= pos && (window <= 0 || p < sink || p > pos - window);
+  return (p <= pos) & ((window <= 0) | (p < sink) | (p > pos - window));
 }
 
 // Every token of [tok, tok + n) is seen by every row of the unit.
 __device__ __forceinline__ bool all_seen(const Attn8Args& A, const Unit8& U, int tok, int n) {
-  return tok + n - 1 <= U.pos0 && (A.window <= 0 || tok + n <= A.sink || tok > U.pos1 - A.window);
+  return (tok + n - 1 <= U.pos0) & ((A.window <= 0) | (tok + n <= A.sink) | (tok > U.pos1 - A.window));
 }
 
 // What a token of the pair's rows weighs by: kf turns q . k into x, lv is
@@ -523,23 +602,25 @@ struct Meta8 {
   float kf, lv, inv;
 };
 
-__device__ __forceinline__ Meta8 meta8(const Attn8Args& A, int b, int head, int tok, bool live) {
-  const Cache8& C = A.C;
-  Meta8 m = {-1, 0.f, 0.f, 1.f};
-  if (live) {
-    const int id = C.bt[(int64_t)b * C.max_blocks + (tok >> C.ps_log2)];
-    if (id >= 0 && id < C.num_pages) {
-      m.page = id;
-      const int64_t at = scale_index(C, id, head, tok);
-      m.kf = C.ks[at] * A.scale_log2;
-      const float vs = C.vs[at];
-      // a scale that is hardly one counts as the writer's least
-      const float s = vs < 0x1p-100f ? 0x1p-100f : vs;
-      m.lv = __builtin_amdgcn_logf(s);
-      m.inv = s == s ? 1.f / s : 1.f;   // a NaN arrives through lv, where masks hold
-    }
+// The table's entry of a token (-1: not live), and the page that it names.
+__device__ __forceinline__ int entry8(const Cache8& C, int b, int tok, bool live) {
+  int id = -1;
+  if (live) id = C.bt[(int64_t)b * C.max_blocks + (tok >> C.ps_log2)];
+  return id;
+}
+__device__ __forceinline__ int page8(const Cache8& C, int id) { return id < C.num_pages ? id : -1; }
+__device__ __forceinline__ float2v scales8(const Cache8& C, int page, int head, int tok) {
+  float2v s = {0.f, 1.f};
+  if (page >= 0) {
+    const int64_t at = scale_index(C, page, head, tok);
+    s = float2v{C.ks[at], C.vs[at]};
   }
-  return m;
+  return s;
+}
+__device__ __forceinline__ Meta8 meta8(const Attn8Args& A, int page, float2v s) {
+  const float vs = s[1] < 0x1p-100f ? 0x1p-100f : s[1];   // a scale that is hardly one counts as the writer's least
+  return Meta8{page, s[0] * A.scale_log2, __builtin_amdgcn_logf(vs),
+               vs == vs ? 1.f / vs : 1.f};                // a NaN arrives through lv, where masks hold
 }
 
 // Place of row `row` of a pair in the output.
@@ -556,35 +637,108 @@ __device__ __forceinline__ void store_out(const Attn8Args& A, int64_t at, float4
 
 // ---- the narrow kernel ----
 //
-// The tiles (32 tokens) of all pairs of a sequence and a KV head, in order, are
-// dealt to the launch's workgroups in equal runs, whatever the sequences'
-// lengths: each finds its run from the lengths on the device.  A pair that
-// falls to several workgroups leaves partial rows in the workspace, which a
-// second kernel joins.
+// A pair is a sequence and `side` neighbouring KV heads, a wave or more each:
+// where the heads' rows of a token are neighbours in memory, the waves read them
+// together (NHD pages, B=32, L=32768: 405 -> 350 us).  The tiles (32 tokens) of
+// all pairs, in order, are dealt to the launch's workgroups in equal runs,
+// whatever the sequences' lengths: each finds its run from the lengths on the
+// device.  A pair that falls to several workgroups leaves partial rows in the
+// workspace, which a second kernel joins.
 
-__device__ __forceinline__ uint32_t wave_total(uint32_t x) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off);
-  return __builtin_amdgcn_readfirstlane(x);
+// The sum of the lanes' x up to this one (DPP: row_shr 1, 2, 4, 8 inside rows of
+// 16 lanes, then row_bcast 15 and 31 across them).
+__device__ __forceinline__ uint32_t upto_lane(uint32_t x) {
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+__device__ __forceinline__ uint32_t last_lane(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
+
+// Tiles of one KV head of sequence u0 + lane.
+__device__ __forceinline__ uint32_t tiles_a(const Attn8Args& A, int64_t v) {
+  return v < A.C.B ? (uint32_t)unit_a(A, v).tiles() : 0u;
 }
 
-// Tiles of all sequences, and of those before sequence u (one KV head's).
-struct Counts8 {
-  int64_t all, before;
-};
-__device__ __forceinline__ Counts8 count8(const Attn8Args& A, int64_t u, int lane) {
-  Counts8 c = {0, 0};
-  for (int64_t u0 = 0; u0 < A.C.B; u0 += 64) {
-    const int64_t v = u0 + lane;
-    const uint32_t n = v < A.C.B ? (uint32_t)unit_a(A, v).tiles() : 0u;
-    c.all += wave_total(n);
-    if (u0 < u) c.before += wave_total(v < u ? n : 0u);
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {   // of numbers >= 0
+  return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
+// How a launch's tiles are dealt (all: one KV head's, some: sequences with any).
+//   side, pairs  KV heads of a pair, and pairs of a sequence.  Heads side by side
+//                where the runs are long, or where a workgroup has several pairs
+//                (fewer of them: 256 sequences of up to 300 tokens 118 -> 57 us);
+//                else a head's waves, joined in the workgroup.
+//   toll         what a pair costs besides its tiles, in tiles, where a
+//                workgroup has several: its loads' latencies, 6 us
+//   share        a workgroup's run of tiles (and tolls)
+//   alone        the runs are short, and the pairs so few that each can be cut
+//                into parts of at most `share` tiles, a workgroup each: no
+//                workgroup then pays a second pair's latencies
+struct Deal8 {
+  int side, pairs, toll;
+  bool alone;
+  int64_t share;
+  // what a pair of n tiles takes of the runs' common line
+  __device__ __forceinline__ int64_t length(uint32_t n) const {
+    if (n == 0) return 0;
+    return alone ? (int64_t)((n + (uint32_t)share - 1) / (uint32_t)share) * share : (int64_t)n + toll;
   }
-  return c;
+};
+constexpr int kLongRun = 16, kLeastRounds = 2;
+// (n: the lane's sequence's tiles, of the first 64)
+__device__ __forceinline__ Deal8 deal8(const Attn8Args& A, int64_t all, int64_t some, uint32_t n) {
+  Deal8 d;
+  const bool crowd = some * A.C.KVH > A.groups;
+  const bool lengthy = all * A.C.KVH >= (int64_t)kLongRun * kWavesA * A.groups;
+  const bool far = lengthy && A.C.head_bytes < (int64_t)A.C.row_bytes;
+  d.side = (crowd | far) ? A.side : 1;
+  d.pairs = A.C.KVH / d.side;
+  const int phases = kWavesA / d.side;
+  const int64_t count = some * d.pairs;
+  d.alone = !lengthy & (2 * count <= A.groups);
+  d.toll = 2 * count > A.groups ? 4 * phases : 0;
+  // runs no shorter than a pair of few tiles, or two tiles for each wave of a head
+  const int64_t least = min(quotient(all + some - 1, max(some, (int64_t)1)), (int64_t)kLeastRounds * phases);
+  const int64_t even = max(quotient((all + some * d.toll) * d.pairs + A.groups - 1, A.groups), max(least, (int64_t)1));
+  d.share = even;
+  if (d.alone) {
+    // all / share parts and one a pair are enough workgroups for certain; with
+    // 64 sequences at most, the least of some shares between that does
+    const int64_t sure = max(quotient(all * d.pairs + A.groups - count - 1, A.groups - count), even);
+    d.share = sure;
+    if (A.C.B <= 64) {
+#pragma unroll
+      for (int k = 2; k >= 0; --k) {
+        const uint32_t t = (uint32_t)(even + (sure - even) * k / 3);
+        const uint32_t parts = last_lane(upto_lane((n + t - 1) / t));
+        if ((int64_t)parts * d.pairs <= A.groups) d.share = t;
+      }
+    }
+  }
+  return d;
 }
 
-__device__ __forceinline__ int64_t group_share(const Attn8Args& A, int64_t all) {
-  return max((all * A.C.KVH + A.groups - 1) / A.groups, (int64_t)kWavesA);
+// The workspace: partial rows, of two runs a workgroup can leave (the end of one
+// pair, `from` its start the beginning of another), up to A.side heads of
+// kRowsA rows each; each row's maximum and sum; and for every sequence and KV
+// head how its rows were left.
+struct Left8 {
+  int first, n;     // workgroups first .. first + n - 1 have parts of the rows; n = 0: written whole
+  int side, h;      // their heads side by side, and which this is
+};
+__device__ __forceinline__ int64_t part_place(int side, int group, bool from, int h, int row) {
+  return ((2 * (int64_t)group + (from ? 1 : 0)) * side + h) * kRowsA + row;
+}
+__host__ __device__ inline int64_t part_rows(int groups, int side) { return (int64_t)2 * groups * side * kRowsA; }
+__device__ __forceinline__ float* part_sums(const Attn8Args& A) {
+  return A.part + part_rows(A.groups, A.side) * kHeadDim;
+}
+__device__ __forceinline__ Left8* part_left(const Attn8Args& A) {
+  return reinterpret_cast<Left8*>(part_sums(A) + 2 * part_rows(A.groups, A.side));
 }
 
 // A wave's running softmax: lane (n, g) has row n; O[cb][r] is channel
@@ -593,6 +747,9 @@ struct State8 {
   float4v O[8];
   float m, l;
 };
+
+constexpr int kRing = 2;     // tiles of a wave on their way
+constexpr int kAhead = 32;   // tiles whose pages and scales a wave holds
 
 struct Raw8 {
   u32x4 k[4], v[4];
@@ -607,49 +764,50 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
   const int t = lane & 15, g = lane >> 4;
   char* slot = lds + wave * kSlotA;
 
-  const int64_t all = count8(A, 0, lane).all;
-  const int64_t share = group_share(A, all);
-  int64_t cur = (int64_t)blockIdx.x * share;
-  const int64_t end = min(cur + share, all * C.KVH);
-  if (cur >= end) return;
-
-  // the sequence of tile `cur`
-  int64_t u = 0, base = 0;   // base: tiles of all heads before unit u
-  for (int64_t u0 = 0; u0 < C.B; u0 += 64) {
-    const int64_t v = u0 + lane;
-    const uint32_t n = v < C.B ? (uint32_t)unit_a(A, v).tiles() : 0u;
-    uint32_t upto = n;       // inclusive prefix
+  // this workgroup's run of tiles, and the sequence that it starts in
+  uint32_t n0 = tiles_a(A, lane);
+  int64_t all = last_lane(upto_lane(n0)), some = __builtin_popcountll(__ballot(n0 != 0));
+  for (int64_t u0 = 64; u0 < C.B; u0 += 256) {   // four loads on their way
+    uint32_t n = 0;
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t y = __shfl_up(upto, off);
-      if (lane >= off) upto += y;
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t mine = tiles_a(A, u0 + 64 * k + lane);
+      some += __builtin_popcountll(__ballot(mine != 0));
+      n += mine;
     }
-    const uint64_t past = __ballot(base + (int64_t)upto * C.KVH > cur);
+    all += last_lane(upto_lane(n));
+  }
+  const Deal8 deal = deal8(A, all, some, n0);
+  const int pairs = deal.pairs, side = deal.side, toll = deal.toll;
+  int64_t cur = (int64_t)blockIdx.x * deal.share;
+  int64_t end = cur + deal.share;
+  int64_t u = 0, base = 0;   // base: where the pair begins that `cur` lies in
+  for (;;) {
+    const uint32_t mine = (uint32_t)deal.length(n0), upto = upto_lane(mine);
+    const uint64_t past = __ballot(base + (int64_t)upto * pairs > cur);
     if (past) {
       const int first = __builtin_ctzll(past);
-      u = u0 + first;
-      base += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(upto - n), first) * C.KVH;
+      base += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), first) * pairs;
+      u += first;
       break;
     }
-    base += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)upto, 63) * C.KVH;
+    base += (int64_t)last_lane(upto) * pairs;
+    u += 64;
+    if (u >= C.B) return;    // no run is left
+    n0 = tiles_a(A, u + lane);
   }
+  Unit8 U = unit_a(A, u);
+  int64_t length = deal.length(U.tiles());
+  int pair = (int)quotient(cur - base, length);
+  base += (int64_t)pair * length;
+  const int phases = kWavesA / side, phase = wave / side;   // waves of a head
 
-  while (cur < end) {
-    const Unit8 U = unit_a(A, u);
+  for (;;) {
     const int nt = U.tiles();
-    if (nt == 0) {
-      ++u;
-      continue;
-    }
-    const int head = (int)((cur - base) / nt);
-    if (head >= C.KVH) {   // the unit's pairs are done
-      base += (int64_t)nt * C.KVH;
-      ++u;
-      continue;
-    }
-    const int j0 = (int)((cur - base) - (int64_t)head * nt);
-    const int j1 = (int)min((int64_t)nt, j0 + (end - cur));
-    cur += j1 - j0;
+    const int j0 = (int)max(cur - base - toll, (int64_t)0);
+    const int j1 = (int)max(min((int64_t)nt, end - base - toll), (int64_t)0);
+    if (j0 < j1) {
+    const int head = pair * side + wave % side;
 
     // this lane's query row
     const int my_row = U.row0 + t;
@@ -676,63 +834,79 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
     const int sink = A.window > 0 ? A.sink : 0;
     const char* kbase = C.k + head * C.head_bytes;
     const char* vbase = C.v + head * C.head_bytes;
-    const int own = (j1 - j0 - wave + kWavesA - 1) / kWavesA;   // this wave's tiles: j0 + wave, + kWavesA, ...
+    const int own = (j1 - j0 - phase + phases - 1) / phases;   // this wave's tiles: j0 + phase, + phases, ...
     const uint32_t off0 = (uint32_t)(lane >> 3) * C.row_bytes + 16u * (lane & 7);
+    auto tok_of = [&](int i) { return kTile * U.tile(j0 + phase + phases * i); };
+    auto lane_f = [](float x, int l) {
+      return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
+    };
+    // Lane 2i + h has half h of the wave's tile i of kAhead: its page and scales;
+    // the page, the raw scales of the next kAhead tiles, and the table's entry of
+    // those after: each is loaded kAhead tiles before it is used.
+    const int my_i = lane >> 1, my_h = 16 * (lane & 1);
+    auto my_tok_of = [&](int i0) { return tok_of(min(i0 + my_i, own - 1)) + my_h; };
+    auto entries = [&](int i0) {
+      const int tok = my_tok_of(i0);
+      return entry8(C, U.s.b, tok, i0 + my_i < own && tok < hi);
+    };
 
-    for (int i0 = 0; i0 < own; i0 += 32) {
-      const int n = min(own - i0, 32);
-      // lane 2i + h: half h of the wave's tile i: its page, scales
-      const int mi = lane >> 1;
-      const int mtok = kTile * U.tile(j0 + wave + kWavesA * (i0 + min(mi, n - 1))) + 16 * (lane & 1);
-      const Meta8 meta = meta8(A, U.s.b, head, mtok, mi < n && mtok < hi);
-      auto lane_f = [](float x, int l) {
-        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
-      };
-      auto tok_of = [&](int i) { return kTile * U.tile(j0 + wave + kWavesA * (i0 + i)); };
+    if (own > 0) {
+      const int first = entries(0), second = entries(kAhead);
+      int after = entries(2 * kAhead), next = -1;
+      Meta8 meta;
+      meta.page = page8(C, first);
+      // (whole halves of pages, also where not every row is seen: no branch, so
+      // that the waits for the loads stay exact)
       auto load = [&](int i, Raw8& X) {
-        const bool live = i < n;
-        const int tok = tok_of(live ? i : 0);
-        const bool full = all_seen(A, U, tok, kTile);
+        const bool live = i < own;
+        const int at = i & (kAhead - 1), row = tok_of(live ? i : 0) & ((1 << C.ps_log2) - 1);
+        const int from = at < kRing && i >= kAhead ? next : meta.page;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int id = live ? __builtin_amdgcn_readlane(meta.page, 2 * i + h) : -1;
-          const uint32_t bytes = id >= 0 ? 15u * C.row_bytes + kCodeRow : 0u;
-          const int64_t off = id >= 0 ? row_offset(C, id, 0, tok + 16 * h) : 0;
+          const int page = __builtin_amdgcn_readlane(from, 2 * at + h);
+          const uint32_t bytes = (live & (page >= 0)) ? 15u * C.row_bytes + kCodeRow : 0u;
+          // a tile's second half is the first's page's next rows, or at a page's start
+          const int64_t off = max(page, 0) * C.page_bytes + (int64_t)((row + 16 * h) & ((1 << C.ps_log2) - 1)) * C.row_bytes;
           const rsrc_t rk = make_rsrc(kbase + off, bytes), rv = make_rsrc(vbase + off, bytes);
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            uint32_t o = off0 + 8u * r * C.row_bytes;
-            if (!full) {   // rows that no query row sees read as zeros
-              const int p = tok + 16 * h + 8 * r + (lane >> 3);
-              if (!(p < hi && (p >= lo || p < sink))) o = kOOB;
-            }
-            X.k[2 * h + r] = bload16(rk, o);
-            X.v[2 * h + r] = bload16(rv, o);
+            X.k[2 * h + r] = bload16(rk, off0 + 8u * r * C.row_bytes);
+            X.v[2 * h + r] = bload16(rv, off0 + 8u * r * C.row_bytes);
           }
         }
       };
+      // i: the tile; its page and scales are lane 2 (i mod kAhead)'s (past the
+      // wave's last tile: one that no row sees)
       auto step = [&](int i, Raw8& X) {
-        const int tok = tok_of(i);
+        const int tok = i < own ? tok_of(i) : 0x7fff0000, at = 2 * (i & (kAhead - 1));
         const bool full = all_seen(A, U, tok, kTile);
-        // staged: K rows' 16-byte chunks turned by the row, V's by its place
-        // among the eight rows that a transposed read takes
         const int r8 = lane >> 3, ch = lane & 7;
         bool nans = false;
+        if (!full) {
+          // V rows that no query row sees count as zeros; a NaN that some see
+          // takes the longer way below
+          uint32_t any = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int p = tok + 8 * k + r8;
+            const bool seen = p < hi && (p >= lo || p < sink);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              X.v[k][d] = seen ? X.v[k][d] : 0u;
+              any |= nan_codes(X.v[k][d]);
+            }
+          }
+          nans = CODE == kE4m3 && __any(any != 0);
+        }
+        // staged: K rows' 16-byte chunks turned by the row, V's by its place
+        // among the eight rows that a transposed read takes
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int r = 8 * k + r8;
           *reinterpret_cast<u32x4*>(slot + r * kCodeRow + ((ch ^ r8) << 4)) = X.k[k];
           *reinterpret_cast<u32x4*>(slot + kTile * kCodeRow + r * kCodeRow + ((ch ^ ((r8 & 3) | ((k >> 1) << 2))) << 4)) = X.v[k];
         }
-        if (CODE == kE4m3 && !full) {
-          uint32_t any = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int d = 0; d < 4; ++d) any |= nan_codes(X.v[k][d]);
-          nans = __any(any != 0);
-        }
-        load(i + 2, X);
+        load(i + kRing, X);
 
         float4v s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -744,15 +918,17 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
           s1 = mfma16x16x32<E>(widen8<CODE, E>(u32x2{b[0], b[1]}), qB[2 * h2], s1);
           s1 = mfma16x16x32<E>(widen8<CODE, E>(u32x2{b[2], b[3]}), qB[2 * h2 + 1], s1);
         }
-        const float kf0 = lane_f(meta.kf, 2 * i), kf1 = lane_f(meta.kf, 2 * i + 1);
-        const float lv0 = lane_f(meta.lv, 2 * i), lv1 = lane_f(meta.lv, 2 * i + 1);
-        const float inv0 = lane_f(meta.inv, 2 * i), inv1 = lane_f(meta.inv, 2 * i + 1);
+        const float kf0 = lane_f(meta.kf, at), kf1 = lane_f(meta.kf, at + 1);
+        const float lv0 = lane_f(meta.lv, at), lv1 = lane_f(meta.lv, at + 1);
+        const float inv0 = lane_f(meta.inv, at), inv1 = lane_f(meta.inv, at + 1);
         float x[8];
-        uint32_t seen = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 8; ++j)
           x[j] = __builtin_fmaf(j < 4 ? s0[j & 3] : s1[j & 3], j < 4 ? kf0 : kf1, j < 4 ? lv0 : lv1);
-          if (!full) {
+        uint32_t seen = 0;
+        if (!full) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
             const bool ok = sees(tok + tau(g, j), pos, A.window, sink);
             seen |= (uint32_t)ok << j;
             x[j] = ok ? x[j] : -INFINITY;
@@ -779,14 +955,16 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
           pL[j] = (_Float16)(w - (float)pB[j]);
         }
         const char* vt = slot + kTile * kCodeRow + tau(g, t >> 1) * kCodeRow + 8 * (t & 1);
+        if (CODE == kE4m3 && nans) {
+          // a NaN reaches the rows that see its token: marked as ones, and
+          // multiplied with what each row sees; the others count it as 0
+          half8 eyes;
 #pragma unroll
-        for (int cb = 0; cb < 8; ++cb) {
-          u32x2 c = lds_read_tr8(vt + ((cb ^ (t >> 1)) << 4));
-          if (CODE == kE4m3 && nans) {
-            // a NaN reaches the rows that see its token: marked as ones, and
-            // multiplied with what each row sees; the others count it as 0
+          for (int j = 0; j < 8; ++j) eyes[j] = (seen >> j) & 1u ? (_Float16)1.f : (_Float16)0.f;
+#pragma unroll
+          for (int cb = 0; cb < 8; ++cb) {
+            u32x2 c = lds_read_tr8(vt + ((cb ^ (t >> 1)) << 4));
             u32x4 marks;
-            half8 eyes;
 #pragma unroll
             for (int d = 0; d < 2; ++d) {
               const uint32_t bad = nan_codes(c[d]) >> 7;   // 0 or 1 a byte
@@ -794,27 +972,47 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
               marks[2 * d] = (bad & 1u) * 0x3c00u | ((bad >> 8) & 1u) * 0x3c000000u;
               marks[2 * d + 1] = ((bad >> 16) & 1u) * 0x3c00u | ((bad >> 24) & 1u) * 0x3c000000u;
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) eyes[j] = (seen >> j) & 1u ? (_Float16)1.f : (_Float16)0.f;
             const float4v hit = mfma16x16x32<kEltF16>(marks, eyes, float4v{0.f, 0.f, 0.f, 0.f});
+            const u32x4 a = widen8<CODE, kEltF16>(c);
+            st.O[cb] = mfma16x16x32<kEltF16>(a, pB, st.O[cb]);
+            st.O[cb] = mfma16x16x32<kEltF16>(a, pL, st.O[cb]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) st.O[cb][r] = hit[r] > 0.f ? __builtin_nanf("") : st.O[cb][r];
           }
-          const u32x4 a = widen8<CODE, kEltF16>(c);
-          st.O[cb] = mfma16x16x32<kEltF16>(a, pB, st.O[cb]);
-          st.O[cb] = mfma16x16x32<kEltF16>(a, pL, st.O[cb]);
+        } else {
+#pragma unroll
+          for (int cb = 0; cb < 8; ++cb) {
+            const u32x4 a = widen8<CODE, kEltF16>(lds_read_tr8(vt + ((cb ^ (t >> 1)) << 4)));
+            st.O[cb] = mfma16x16x32<kEltF16>(a, pB, st.O[cb]);
+            st.O[cb] = mfma16x16x32<kEltF16>(a, pL, st.O[cb]);
+          }
         }
       };
       Raw8 X0, X1;
       load(0, X0);
       load(1, X1);
-      for (int i = 0; i < n; i += 2) {
-        step(i, X0);
-        if (i + 1 < n) step(i + 1, X1);
+      {
+        const float2v now = scales8(C, meta.page, head, my_tok_of(0));
+        next = page8(C, second);
+        meta = meta8(A, meta.page, now);
+      }
+      float2v next_s = scales8(C, next, head, my_tok_of(kAhead));
+      for (int i0 = 0;;) {
+        const int i1 = min(i0 + kAhead, own);
+        for (int i = i0; i < i1; i += kRing) {
+          step(i, X0);
+          step(i + 1, X1);
+        }
+        i0 = i1;
+        if (i0 >= own) break;
+        meta = meta8(A, next, next_s);
+        next = page8(C, after);
+        next_s = scales8(C, next, head, my_tok_of(i0 + kAhead));
+        after = entries(i0 + 2 * kAhead);
       }
     }
 
-    // join the waves: each parks its rows in its slot
+    // join the waves of a head: each parks its rows in its slot
     const float l = group_sum(st.l);
     if (g == 0) {
       lds_m[wave][t] = st.m;
@@ -824,92 +1022,150 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
     for (int cb = 0; cb < 8; ++cb)
       *reinterpret_cast<float4v*>(slot + t * (kHeadDim * 4) + (((4 * cb + g) ^ t) << 4)) = st.O[cb];
     __syncthreads();
-    {
-      const int row = threadIdx.x >> 4;   // kThreadsA / 16 == kRowsA
-      float M = lds_m[0][row], f[kWavesA], L = 0.f;
-#pragma unroll
-      for (int w = 1; w < kWavesA; ++w) M = fmaxf(M, lds_m[w][row]);
-#pragma unroll
-      for (int w = 0; w < kWavesA; ++w) {
-        f[w] = __builtin_amdgcn_exp2f(lds_m[w][row] - M);
-        L = __builtin_fmaf(lds_l[w][row], f[w], L);
-      }
-      const bool whole = j1 - j0 == nt;
-      const int64_t place = 2 * (int64_t)blockIdx.x + (j0 == 0 ? 1 : 0);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int chunk = (threadIdx.x & 15) + 16 * h;
-        float4v acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kWavesA; ++w)
-          acc += *reinterpret_cast<const float4v*>(lds + w * kSlotA + row * (kHeadDim * 4) + ((chunk ^ row) << 4)) * f[w];
-        if (row < U.rows) {
-          if (whole) {
-            store_out<E>(A, out_row(A, U, head, row) + 4 * chunk, acc, L);
-          } else {
-            *reinterpret_cast<float4v*>(A.part + (place * kRowsA + row) * kHeadDim + 4 * chunk) = acc;
-          }
+    const bool whole = j1 - j0 == nt;
+    const int row = threadIdx.x >> 4;   // kThreadsA / 16 == kRowsA
+    if (row < U.rows) {
+      for (int h = 0; h < side; ++h) {
+        float M = lds_m[h][row], L = 0.f;
+        for (int w = h + side; w < kWavesA; w += side) M = fmaxf(M, lds_m[w][row]);
+        float4v acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        const int chunk = threadIdx.x & 15;
+        for (int w = h; w < kWavesA; w += side) {
+          const float f = __builtin_amdgcn_exp2f(lds_m[w][row] - M);
+          L = __builtin_fmaf(lds_l[w][row], f, L);
+          const char* rows = lds + w * kSlotA + row * (kHeadDim * 4);
+          acc[0] += *reinterpret_cast<const float4v*>(rows + ((chunk ^ row) << 4)) * f;
+          acc[1] += *reinterpret_cast<const float4v*>(rows + (((chunk + 16) ^ row) << 4)) * f;
         }
-      }
-      if (!whole && row < U.rows && (threadIdx.x & 15) == 0) {
-        float* ml = A.part + (int64_t)2 * A.groups * kRowsA * kHeadDim;
-        ml[place * kRowsA + row] = M;
-        ml[(int64_t)2 * A.groups * kRowsA + place * kRowsA + row] = L;
+        const int hd = pair * side + h;
+        const int64_t place = part_place(side, blockIdx.x, j0 == 0, h, row);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (whole)
+            store_out<E>(A, out_row(A, U, hd, row) + 4 * (chunk + 16 * k), acc[k], L);
+          else
+            *reinterpret_cast<float4v*>(A.part + place * kHeadDim + 4 * (chunk + 16 * k)) = acc[k];
+        }
+        if (!whole && chunk == 0) *reinterpret_cast<float2v*>(part_sums(A) + 2 * place) = float2v{M, L};
       }
     }
+    if (j0 == 0 && (int)threadIdx.x < side) {   // the pair's first run says where the others are
+      Left8 left = {(int)blockIdx.x, 0, side, (int)threadIdx.x};
+      if (!whole) left.n = 1 + (int)quotient(nt - j1 + deal.share - 1, deal.share);
+      part_left(A)[u * C.KVH + pair * side + threadIdx.x] = left;
+    }
+    }
+    base += length;
+    cur = base;
+    if (cur >= end) return;
     __syncthreads();   // the slots are free again
+    if (++pair == pairs) {
+      pair = 0;
+      do {
+        if (++u >= C.B) return;   // the last run may be short
+        U = unit_a(A, u);
+      } while (U.tiles() == 0);
+      length = deal.length(U.tiles());
+    }
   }
 }
 
-// One workgroup a pair's row: the rows that several workgroups share, and
-// zeros for those that attend to nothing.
-template <int E>
+// Joins the rows that several workgroups share, and writes zeros for those that
+// attend to nothing: a workgroup for 16 rows of a sequence and KV head (MANY:
+// enough pairs to fill the GPU, and so few parts of each), or for one row, whose
+// parts it reads eight at a time.
+template <int E, bool MANY>
 __global__ __launch_bounds__(256) void join8_kernel(Attn8Args A) {
   const Cache8& C = A.C;
-  const int lane = threadIdx.x & 63;
-  const int64_t id = blockIdx.x;
-  const int row = (int)(id % kRowsA);
-  const int64_t pair = id / kRowsA, u = pair / C.KVH;
-  const int head = (int)(pair - u * C.KVH);
-  const Unit8 U = unit_a(A, u);
-  if (row >= U.rows) return;
-  const int64_t out = out_row(A, U, head, row);
-  const int nt = U.tiles();
-  if (nt == 0) {
-    if (threadIdx.x < 32) store_out<E>(A, out + 4 * threadIdx.x, float4v{0.f, 0.f, 0.f, 0.f}, 0.f);
-    return;
-  }
-  const Counts8 c = count8(A, u, lane);
-  const int64_t share = group_share(A, c.all);
-  const int64_t begin = c.before * C.KVH + (int64_t)head * nt;
-  const int64_t w0 = begin / share, w1 = (begin + nt - 1) / share;
-  if (w0 == w1) return;   // written whole
-  const float* pm = A.part + (int64_t)2 * A.groups * kRowsA * kHeadDim;
-  const float* pl = pm + (int64_t)2 * A.groups * kRowsA;
-  auto place = [&](int64_t w) { return (2 * w + (w == w0 ? 1 : 0)) * kRowsA + row; };
-  float M = kMaxSentinel;
-  for (int64_t w = w0; w <= w1; ++w) M = fmaxf(M, pm[place(w)]);
   const int grp = threadIdx.x >> 5, chunk = threadIdx.x & 31;
-  float4v acc = {0.f, 0.f, 0.f, 0.f};
-  float L = 0.f;
-  for (int64_t w = w0 + grp; w <= w1; w += 8) {
-    const int64_t p = place(w);
-    const float f = __builtin_amdgcn_exp2f(pm[p] - M);
-    L = __builtin_fmaf(pl[p], f, L);
-    acc += *reinterpret_cast<const float4v*>(A.part + p * kHeadDim + 4 * chunk) * f;
-  }
-  __shared__ float4v parts[8][32];
-  __shared__ float sums[8];
-  parts[grp][chunk] = acc;
-  if (chunk == 0) sums[grp] = L;
-  __syncthreads();
-  if (grp != 0) return;
+  const uint32_t id = MANY ? blockIdx.x : blockIdx.x / (uint32_t)kRowsA;
+  const int head = (int)(id % (uint32_t)C.KVH);
+  const int64_t u = id / (uint32_t)C.KVH;
+  const Left8 left = part_left(A)[id];
+  const Unit8 U = unit_a(A, u);
+  const bool none = U.tiles() == 0;        // (then nothing is said of its rows)
+  if (!none && left.n == 0) return;
+  // the parts of a row: a first run's is its second place, the others' the first
+  auto part = [&](int i, int row) { return part_place(left.side, left.first + i, i == 0, left.h, row); };
+  const float2v* sums = reinterpret_cast<const float2v*>(part_sums(A));
+  if constexpr (MANY) {
+    for (int row = grp; row < U.rows; row += 8) {
+      float M = kMaxSentinel, L = 0.f;
+      float4v acc = {0.f, 0.f, 0.f, 0.f};
+      for (int i0 = 0; !none && i0 < left.n; i0 += 8) {
+        float2v ml[8];
+        float4v a[8];
+        float top = M;
 #pragma unroll
-  for (int w = 1; w < 8; ++w) {
-    acc += parts[w][chunk];
-    L += sums[w];
+        for (int k = 0; k < 8; ++k) {
+          const int64_t p = part(min(i0 + k, left.n - 1), row);
+          ml[k] = sums[p];
+          a[k] = *reinterpret_cast<const float4v*>(A.part + p * kHeadDim + 4 * chunk);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k][0]);
+        const float again = __builtin_amdgcn_exp2f(M - top);
+        M = top;
+        acc = acc * again;
+        L *= again;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (i0 + k < left.n) {
+            const float f = __builtin_amdgcn_exp2f(ml[k][0] - M);
+            acc += a[k] * f;
+            L = __builtin_fmaf(ml[k][1], f, L);
+          }
+      }
+      store_out<E>(A, out_row(A, U, head, row) + 4 * chunk, acc, L);
+    }
+  } else {
+    const int row = (int)(blockIdx.x % (uint32_t)kRowsA);
+    if (row >= U.rows) return;
+    float M = kMaxSentinel, L = 0.f;
+    float4v acc = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = grp; !none && i0 < left.n; i0 += 32) {   // parts grp, + 8, ..., four on their way
+      float2v ml[4];
+      float4v a[4];
+      float top = M;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t p = part(min(i0 + 8 * k, left.n - 1), row);
+        ml[k] = sums[p];
+        a[k] = *reinterpret_cast<const float4v*>(A.part + p * kHeadDim + 4 * chunk);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = fmaxf(top, ml[k][0]);
+      const float again = __builtin_amdgcn_exp2f(M - top);
+      M = top;
+      acc = acc * again;
+      L *= again;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i0 + 8 * k < left.n) {
+          const float f = __builtin_amdgcn_exp2f(ml[k][0] - M);
+          acc += a[k] * f;
+          L = __builtin_fmaf(ml[k][1], f, L);
+        }
+    }
+    __shared__ float4v rows[8][32];
+    __shared__ float2v both[8];
+    rows[grp][chunk] = acc;
+    if (chunk == 0) both[grp] = float2v{M, L};
+    __syncthreads();
+    if (grp != 0) return;
+    float top = M;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) top = fmaxf(top, both[w][0]);
+    acc = float4v{0.f, 0.f, 0.f, 0.f};
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const float f = __builtin_amdgcn_exp2f(both[w][0] - top);
+      acc += rows[w][chunk] * f;
+      L = __builtin_fmaf(both[w][1], f, L);
+    }
+    store_out<E>(A, out_row(A, U, head, row) + 4 * chunk, acc, L);
   }
-  store_out<E>(A, out + 4 * chunk, acc, L);
 }
 
 // ---- the wide kernel ----
@@ -1026,7 +1282,8 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
     {
       const int i = threadIdx.x / kSegs;
       const int tok = kTileB * U.tile(i0 + min(i, cnt - 1)) + 16 * (threadIdx.x % kSegs);
-      metas[threadIdx.x] = meta8(A, U.s.b, head, tok, i < cnt && tok < hi);
+      const int page = page8(C, entry8(C, U.s.b, tok, i < cnt && tok < hi));
+      metas[threadIdx.x] = meta8(A, page, scales8(C, page, head, tok));
       if (threadIdx.x < 4) nan_seen[threadIdx.x] = 0;
     }
     __syncthreads();
@@ -1323,12 +1580,18 @@ int launch_read(const Read8Args& A, int dtype, hipStream_t stream) {
 
 // Narrow kernel: workgroups, no more than there can be runs of one tile a wave;
 // none if no sequence can have so few rows.
-int narrow_groups(bool offsets, int64_t B, int32_t KVH, int32_t G, int64_t max_len) {
+int narrow_groups(int64_t B, int32_t KVH, int32_t G, int64_t max_len) {
   if (G > kRowsA) return 0;
   const int64_t tiles = B * KVH * ((max_len + kTile - 1) / kTile);
   return (int)std::min<int64_t>(kGroupsA, std::max<int64_t>(1, (tiles + kWavesA - 1) / kWavesA));
 }
-size_t narrow_bytes(int groups) { return (size_t)2 * groups * kRowsA * (kHeadDim + 2) * sizeof(float); }
+size_t narrow_bytes(int groups, int side, int64_t heads) {
+  return groups ? (size_t)part_rows(groups, side) * (kHeadDim + 2) * sizeof(float) + (size_t)heads * sizeof(Left8) : 0;
+}
+// KV heads that a workgroup reads side by side.
+int narrow_side(int32_t KVH) { return KVH % 4 == 0 ? 4 : KVH % 2 == 0 ? 2 : 1; }
+
+constexpr int kManyPairs = 64;   // from here on the pairs' parts are few (eight or so)
 
 // Wide kernel: units of a call (with those of the rows past the last sequence),
 // and splits a pair where the pairs do not fill the GPU.
@@ -1346,7 +1609,7 @@ size_t wide_bytes(int64_t units, int32_t KVH, int splits) {
 
 size_t attn_bytes(bool offsets, int64_t B, int64_t T, int32_t G, int32_t KVH, int64_t max_len) {
   const int64_t units = wide_units(offsets, B, T, G);
-  return std::max(narrow_bytes(narrow_groups(offsets, B, KVH, G, max_len)),
+  return std::max(narrow_bytes(narrow_groups(B, KVH, G, max_len), narrow_side(KVH), B * KVH),
                   wide_bytes(units, KVH, wide_splits(units, KVH, max_len)));
 }
 
@@ -1355,7 +1618,11 @@ int launch_attn8(Attn8Args A, hipStream_t stream) {
   // one after the other: both kernels' partial rows go to the same workspace
   if (A.groups > 0) {
     attn8_kernel<CODE, E><<<dim3((unsigned)A.groups), dim3(kThreadsA), 0, stream>>>(A);
-    join8_kernel<E><<<dim3((unsigned)(A.C.B * A.C.KVH * kRowsA)), dim3(256), 0, stream>>>(A);
+    const int64_t heads = A.C.B * A.C.KVH;
+    if (heads / A.side >= kManyPairs)
+      join8_kernel<E, true><<<dim3((unsigned)heads), dim3(256), 0, stream>>>(A);
+    else
+      join8_kernel<E, false><<<dim3((unsigned)(heads * kRowsA)), dim3(256), 0, stream>>>(A);
     const int rc = launch_status();
     if (rc) return rc;
   }
@@ -1431,7 +1698,8 @@ int kvdec_paged8_attention(const kvdec_paged8_cache* cache, const void* q, void*
   if (window < 0 || sink < 0 || (window == 0 && sink > 0)) return KVDEC_E_WINDOW;
   if (!on16(q) || !on16(o) || q_token_stride % 8 || q_head_stride % 8) return KVDEC_E_UNSUPPORTED;
   const bool offsets = cu_seqlens != nullptr;
-  A.groups = narrow_groups(offsets, B, A.C.KVH, A.G, A.C.max_len);
+  A.groups = narrow_groups(B, A.C.KVH, A.G, A.C.max_len);
+  A.side = narrow_side(A.C.KVH);
   A.units = wide_units(offsets, B, T, A.G);
   A.splits = wide_splits(A.units, A.C.KVH, A.C.max_len);
   if (B * A.C.KVH * kRowsA > 0x7fffffff || A.units * A.C.KVH * std::max(A.splits, kRowsB / 8) > 0x7fffffff)
