@@ -1228,6 +1228,7 @@ template <int CODE, int E>
 __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
   __shared__ __align__(16) char ks[2][kTileBytesB], vs[2][kTileBytesB];
   __shared__ Meta8 metas[kThreadsB];
+  __shared__ __align__(16) uint2 places[kThreadsB];   // a segment's bytes from the KV head's first, or (y < 0) none
   // e4m3, tiles that not every row sees whole: whether V tile i & 3 has a NaN,
   // and which channels of each token
   __shared__ int nan_seen[4];
@@ -1274,7 +1275,8 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
   const int sink = A.window > 0 ? A.sink : 0;
   const char* kbase = C.k + head * C.head_bytes;
   const char* vbase = C.v + head * C.head_bytes;
-  const int r4 = lane >> 4, ch = lane & 15;   // staging: row 16 i + 4 wave + r4, 8 codes from 8 ch
+  const int r4 = lane >> 4, ch = lane & 15;   // staging: row 16 g + 4 wave + r4, 8 codes from 8 ch
+  const uint32_t off0 = (uint32_t)(4 * wave + r4) * C.row_bytes + 8u * ch;
 
   for (int i0 = j0; i0 < j1; i0 += kChunkB) {
     const int cnt = min(j1 - i0, kChunkB);
@@ -1284,49 +1286,54 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
       const int tok = kTileB * U.tile(i0 + min(i, cnt - 1)) + 16 * (threadIdx.x % kSegs);
       const int page = page8(C, entry8(C, U.s.b, tok, i < cnt && tok < hi));
       metas[threadIdx.x] = meta8(A, page, scales8(C, page, head, tok));
+      const uint64_t off = page >= 0 ? (uint64_t)row_offset(C, page, 0, tok) : ~0ull;
+      places[threadIdx.x] = uint2{(uint32_t)off, (uint32_t)(off >> 32)};
       if (threadIdx.x < 4) nan_seen[threadIdx.x] = 0;
     }
     __syncthreads();
 
     u32x2 kc[kSegs], vc[kSegs];   // codes on their way: of the tile after the next
+    // (whole segments, also where not every row is seen: no branch, so that the
+    // waits for the loads stay exact)
     auto load = [&](int i) {
       const bool live = i < cnt;
-      const int tok = kTileB * U.tile(i0 + (live ? i : 0));
-      const bool full = all_seen(A, U, tok, kTileB);
+      const uint2* at = places + kSegs * min(i, kChunkB - 1);
 #pragma unroll
       for (int g = 0; g < kSegs; ++g) {
-        const int page = live ? __builtin_amdgcn_readfirstlane(metas[kSegs * i + g].page) : -1;
-        const uint32_t bytes = page >= 0 ? 15u * C.row_bytes + kCodeRow : 0u;
-        const int64_t off = page >= 0 ? row_offset(C, page, 0, tok + 16 * g) : 0;
-        uint32_t o = (uint32_t)(4 * wave + r4) * C.row_bytes + 8u * ch;
-        if (!full) {   // rows that no query row sees read as zeros
-          const int p = tok + 16 * g + 4 * wave + r4;
-          if (!(p < hi && (p >= lo || p < sink))) o = kOOB;
-        }
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)at[g].x);
+        const int hi32 = __builtin_amdgcn_readfirstlane((int)at[g].y);
+        const uint32_t bytes = (live & (hi32 >= 0)) ? 15u * C.row_bytes + kCodeRow : 0u;
+        const uint64_t off = ((uint64_t)(uint32_t)max(hi32, 0) << 32) | lo;
         typedef int v2i __attribute__((ext_vector_type(2)));
-        kc[g] = __builtin_bit_cast(u32x2, (v2i)__builtin_amdgcn_raw_buffer_load_b64(make_rsrc(kbase + off, bytes), o, 0, 0));
-        vc[g] = __builtin_bit_cast(u32x2, (v2i)__builtin_amdgcn_raw_buffer_load_b64(make_rsrc(vbase + off, bytes), o, 0, 0));
+        kc[g] = __builtin_bit_cast(u32x2, (v2i)__builtin_amdgcn_raw_buffer_load_b64(make_rsrc(kbase + off, bytes), off0, 0, 0));
+        vc[g] = __builtin_bit_cast(u32x2, (v2i)__builtin_amdgcn_raw_buffer_load_b64(make_rsrc(vbase + off, bytes), off0, 0, 0));
       }
     };
     auto stage = [&](int i) {
       const int buf = i & 1;
-      // a NaN of V must not meet the weight 0 of a row that does not see it: it
-      // is staged as 0 and noted
-      if (CODE == kE4m3 && i < cnt && !all_seen(A, U, kTileB * U.tile(i0 + i), kTileB)) {
+      const int tok = kTileB * U.tile(i0 + min(i, cnt - 1));
+      if (!all_seen(A, U, tok, kTileB)) {
+        // V rows that no query row sees count as zeros; a NaN must not meet the
+        // weight 0 of a row that does not see it: it is staged as 0 and noted
         uint32_t any = 0;
 #pragma unroll
         for (int g = 0; g < kSegs; ++g) {
+          const int r = 16 * g + 4 * wave + r4, p = tok + r;
+          const bool seen = (p < hi) & ((p >= lo) | (p < sink));
           uint32_t bits = 0;
 #pragma unroll
           for (int d = 0; d < 2; ++d) {
-            const uint32_t bad = nan_codes(vc[g][d]) >> 7;   // 0 or 1 a byte
-            vc[g][d] &= ~(bad * 0xffu);
-            bits |= ((bad * 0x01020408u) >> 24) << (4 * d);
+            vc[g][d] = seen ? vc[g][d] : 0u;
+            if (CODE == kE4m3) {
+              const uint32_t bad = nan_codes(vc[g][d]) >> 7;   // 0 or 1 a byte
+              vc[g][d] &= ~(bad * 0xffu);
+              bits |= ((bad * 0x01020408u) >> 24) << (4 * d);
+            }
           }
-          nan_map[buf][16 * g + 4 * wave + r4][ch] = (uint8_t)bits;
+          if (CODE == kE4m3) nan_map[buf][r][ch] = (uint8_t)bits;
           any |= bits;
         }
-        if (__any(any != 0)) nan_seen[i & 3] = 1;
+        if (CODE == kE4m3 && __any(any != 0)) nan_seen[i & 3] = 1;
       }
 #pragma unroll
       for (int g = 0; g < kSegs; ++g) {
@@ -1370,14 +1377,22 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
           const float add = mt.lv - ref;
 #pragma unroll
           for (int r = 8 * (g & 1); r < 8 * (g & 1) + 8; ++r) {
-            float x = __builtin_fmaf(S[g >> 1][r], mt.kf, add);
-            if (!full) {
-              x = sees(tok + 32 * (g >> 1) + 8 * (r >> 2) + 4 * hf + (r & 3), pos, A.window, A.sink) ? x : -INFINITY;
-            }
-            top = fmaxf(top, x);
-            S[g >> 1][r] = x;
+            S[g >> 1][r] = __builtin_fmaf(S[g >> 1][r], mt.kf, add);
           }
         }
+        if (!full) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int p = tok + 32 * b + 8 * (r >> 2) + 4 * hf + (r & 3);
+              S[b][r] = sees(p, pos, A.window, A.sink) ? S[b][r] : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, S[b][r]);
         if (__any(top > (m == -INFINITY ? -INFINITY : kRescaleSlack))) {
           const float t = half_max(top);
           const float now = m == -INFINITY ? t : fmaxf(m, m + t);
