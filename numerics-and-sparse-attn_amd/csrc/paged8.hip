@@ -1255,7 +1255,6 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
   const int my_tok = (U.row0 + my_row) / A.G, my_head = U.row0 + my_row - my_tok * A.G;
   const bool mine = my_row < U.rows;
   const int pos = mine ? U.s.len - U.s.n + my_tok : -1;
-  const bool busy = 32 * wave < U.rows;   // the wave has rows
   u32x4 qB[8];
 #pragma unroll
   for (int s = 0; s < 8; ++s) {
@@ -1275,8 +1274,11 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
   const int sink = A.window > 0 ? A.sink : 0;
   const char* kbase = C.k + head * C.head_bytes;
   const char* vbase = C.v + head * C.head_bytes;
-  const int r4 = lane >> 4, ch = lane & 15;   // staging: row 16 g + 4 wave + r4, 8 codes from 8 ch
-  const uint32_t off0 = (uint32_t)(4 * wave + r4) * C.row_bytes + 8u * ch;
+  // staging: row 16 g + r16, 8 codes from 8 ch
+  const int r16 = 4 * wave + (lane >> 4), ch = lane & 15;
+  uint32_t off0 = (uint32_t)r16 * C.row_bytes + 8u * ch;
+  uint32_t k_at = r16 * kRowB + ((ch ^ r16) << 4), v_at = r16 * kRowB + ((ch ^ ((r16 & 3) << 2)) << 4);
+  asm volatile("" : "+v"(off0), "+v"(k_at), "+v"(v_at));   // kept, not computed again for each tile
 
   for (int i0 = j0; i0 < j1; i0 += kChunkB) {
     const int cnt = min(j1 - i0, kChunkB);
@@ -1295,22 +1297,17 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
     u32x2 kc[kSegs], vc[kSegs];   // codes on their way: of the tile after the next
     // (whole segments, also where not every row is seen: no branch, so that the
     // waits for the loads stay exact)
-    auto load = [&](int i) {
-      const bool live = i < cnt;
-      const uint2* at = places + kSegs * min(i, kChunkB - 1);
-#pragma unroll
-      for (int g = 0; g < kSegs; ++g) {
-        const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)at[g].x);
-        const int hi32 = __builtin_amdgcn_readfirstlane((int)at[g].y);
-        const uint32_t bytes = (live & (hi32 >= 0)) ? 15u * C.row_bytes + kCodeRow : 0u;
-        const uint64_t off = ((uint64_t)(uint32_t)max(hi32, 0) << 32) | lo;
-        typedef int v2i __attribute__((ext_vector_type(2)));
-        kc[g] = __builtin_bit_cast(u32x2, (v2i)__builtin_amdgcn_raw_buffer_load_b64(make_rsrc(kbase + off, bytes), off0, 0, 0));
-        vc[g] = __builtin_bit_cast(u32x2, (v2i)__builtin_amdgcn_raw_buffer_load_b64(make_rsrc(vbase + off, bytes), off0, 0, 0));
-      }
+    auto load = [&](int i, int g) {
+      const uint2 at = places[kSegs * min(i, kChunkB - 1) + g];
+      const uint32_t lo32 = (uint32_t)__builtin_amdgcn_readfirstlane((int)at.x);
+      const int hi32 = __builtin_amdgcn_readfirstlane((int)at.y);
+      const uint32_t bytes = ((i < cnt) & (hi32 >= 0)) ? 15u * C.row_bytes + kCodeRow : 0u;
+      const uint64_t off = ((uint64_t)(uint32_t)max(hi32, 0) << 32) | lo32;
+      typedef int v2i __attribute__((ext_vector_type(2)));
+      kc[g] = __builtin_bit_cast(u32x2, (v2i)__builtin_amdgcn_raw_buffer_load_b64(make_rsrc(kbase + off, bytes), off0, 0, 0));
+      vc[g] = __builtin_bit_cast(u32x2, (v2i)__builtin_amdgcn_raw_buffer_load_b64(make_rsrc(vbase + off, bytes), off0, 0, 0));
     };
-    auto stage = [&](int i) {
-      const int buf = i & 1;
+    auto mend = [&](int i) {
       const int tok = kTileB * U.tile(i0 + min(i, cnt - 1));
       if (!all_seen(A, U, tok, kTileB)) {
         // V rows that no query row sees count as zeros; a NaN must not meet the
@@ -1318,7 +1315,7 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
         uint32_t any = 0;
 #pragma unroll
         for (int g = 0; g < kSegs; ++g) {
-          const int r = 16 * g + 4 * wave + r4, p = tok + r;
+          const int r = 16 * g + r16, p = tok + r;
           const bool seen = (p < hi) & ((p >= lo) | (p < sink));
           uint32_t bits = 0;
 #pragma unroll
@@ -1330,43 +1327,58 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
               bits |= ((bad * 0x01020408u) >> 24) << (4 * d);
             }
           }
-          if (CODE == kE4m3) nan_map[buf][r][ch] = (uint8_t)bits;
+          if (CODE == kE4m3) nan_map[i & 1][r][ch] = (uint8_t)bits;
           any |= bits;
         }
         if (CODE == kE4m3 && __any(any != 0)) nan_seen[i & 3] = 1;
       }
-#pragma unroll
-      for (int g = 0; g < kSegs; ++g) {
-        const int r = 16 * g + 4 * wave + r4;
-        *reinterpret_cast<u32x4*>(ks[buf] + r * kRowB + ((ch ^ (r & 15)) << 4)) = widen8<CODE, E>(kc[g]);
-        *reinterpret_cast<u32x4*>(vs[buf] + r * kRowB + ((ch ^ ((r & 3) << 2)) << 4)) = widen8<CODE, kEltF16>(vc[g]);
-      }
+    };
+    auto stage_k = [&](int i, int g) {
+      *reinterpret_cast<u32x4*>(ks[i & 1] + k_at + 16 * g * kRowB) = widen8<CODE, E>(kc[g]);
+    };
+    auto stage_v = [&](int i, int g) {
+      *reinterpret_cast<u32x4*>(vs[i & 1] + v_at + 16 * g * kRowB) = widen8<CODE, kEltF16>(vc[g]);
     };
 
-    load(0);
-    stage(0);
-    load(1);
+#pragma unroll
+    for (int g = 0; g < kSegs; ++g) load(0, g);
+    mend(0);
+#pragma unroll
+    for (int g = 0; g < kSegs; ++g) {
+      stage_k(0, g);
+      stage_v(0, g);
+      load(1, g);
+    }
     __syncthreads();
     for (int i = 0; i < cnt; ++i) {
       const int tok = kTileB * U.tile(i0 + i);
       const bool full = all_seen(A, U, tok, kTileB);
       const bool nans = CODE == kE4m3 && !full && nan_seen[i & 3];
       if (CODE == kE4m3 && threadIdx.x == 0) nan_seen[(i + 2) & 3] = 0;
-      stage(i + 1);   // (past the last tile: zeros)
-      load(i + 2);
-      if (busy) {
-        float16v S[2];
-        const char* kt = ks[i & 1];
-        const char* vt = vs[i & 1];
+      mend(i + 1);
+      // this tile's S = K Q^T, and meanwhile the next one staged (past the last:
+      // zeros) and the one behind it loaded
+      float16v S[2];
+      const char* kt = ks[i & 1];
+      const char* vt = vs[i & 1];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) S[b][r] = 0.f;
+        for (int r = 0; r < 16; ++r) S[b][r] = 0.f;
 #pragma unroll
-          for (int s = 0; s < 8; ++s)
-            S[b] = mfma32x32x16<E>(*reinterpret_cast<const u32x4*>(kt + (32 * b + n) * kRowB + (((2 * s + hf) ^ (n & 15)) << 4)),
-                                   qB[s], S[b]);
+      for (int s = 0; s < 8; ++s) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          S[b] = mfma32x32x16<E>(*reinterpret_cast<const u32x4*>(kt + (32 * b + n) * kRowB + (((2 * s + hf) ^ (n & 15)) << 4)),
+                                 qB[s], S[b]);
+        if (s & 1) {
+          stage_v(i + 1, s >> 1);
+          load(i + 2, s >> 1);
+        } else {
+          stage_k(i + 1, s >> 1);
         }
+      }
+      {
         // logits against the running maximum (0 while there is none)
         const float ref = m == -INFINITY ? 0.f : m;
         float inv[kSegs], top = -INFINITY;
