@@ -1422,7 +1422,10 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
             for (int r = 0; r < 16; ++r) O[cb][r] *= f;
           m = now;
         }
-        u32x4 P[kSegs];
+        // lane (group of 16 lanes, 4j + h): row 4 hf + j, channel 16 (group & 1) + 4 h
+        const int j = (lane >> 2) & 3;
+        const char* vl = vt + (4 * hf + j) * kRowB + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+        // 16 tokens' weights, then their products, under which the next 16's are made
 #pragma unroll
         for (int g = 0; g < kSegs; ++g) {
           half8 h;
@@ -1434,20 +1437,13 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
             h[r] = (_Float16)w;
           }
           l = __builtin_fmaf(sum, inv[g], l);
-          P[g] = as_u4(h);
+#pragma unroll
+          for (int cb = 0; cb < 4; ++cb) {
+            const u32x2 a = lds_read_tr16(vl + 16 * g * kRowB + ((cb ^ j) << 6));
+            const u32x2 b = lds_read_tr16(vl + (16 * g + 8) * kRowB + ((cb ^ j) << 6));
+            O[cb] = mfma32x32x16<kEltF16>(u32x4{a[0], a[1], b[0], b[1]}, as_u4(h), O[cb]);
+          }
         }
-        // lane (group of 16 lanes, 4j + h): row 4 hf + j, channel 16 (group & 1) + 4 h
-        const int j = (lane >> 2) & 3;
-        const char* vl = vt + (4 * hf + j) * kRowB + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-        auto values = [&](int g, int cb) {
-          const u32x2 a = lds_read_tr16(vl + 16 * g * kRowB + ((cb ^ j) << 6));
-          const u32x2 b = lds_read_tr16(vl + (16 * g + 8) * kRowB + ((cb ^ j) << 6));
-          return u32x4{a[0], a[1], b[0], b[1]};
-        };
-#pragma unroll
-        for (int cb = 0; cb < 4; ++cb)
-#pragma unroll
-          for (int g = 0; g < kSegs; ++g) O[cb] = mfma32x32x16<kEltF16>(values(g, cb), P[g], O[cb]);
         if (nans) {   // and reaches the rows that do
           u32x4 hit = {0u, 0u, 0u, 0u};   // this row's channels
           for (int p = 0; p < kTileB; ++p)
