@@ -501,13 +501,15 @@ struct Attn8Args {
   Cache8 C;
   const void* q;
   void* o;
-  float* part;                // partial rows, then their maxima and sums
+  float* part;                // the workspace: the narrow kernel's parts,
+  int64_t wide_at;            // and (from this float on) the wide one's
   int64_t q_tok, q_head;      // in elements
   int64_t units;
   int32_t G, H, window, sink;
   int32_t groups;             // narrow: workgroups,
   int32_t side;               // and KV heads that one may read side by side (1, 2 or 4)
-  int32_t splits;             // wide: workgroups a pair
+  int32_t splits;             // wide: workgroups a pair,
+  uint32_t wide_blocks;       // and those of the join
   float scale_log2;
 };
 
@@ -755,10 +757,16 @@ struct Raw8 {
   u32x4 k[4], v[4];
 };
 
+struct NarrowLds {
+  char slots[kWavesA * kSlotA];
+  float m[kWavesA][kRowsA], l[kWavesA][kRowsA];
+};
+
 template <int CODE, int E>
-__global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
-  __shared__ __align__(16) char lds[kWavesA * kSlotA];
-  __shared__ float lds_m[kWavesA][kRowsA], lds_l[kWavesA][kRowsA];
+__device__ __forceinline__ void narrow_part(const Attn8Args& A, int group, NarrowLds& L8) {
+  char* const lds = L8.slots;
+  auto& lds_m = L8.m;
+  auto& lds_l = L8.l;
   const Cache8& C = A.C;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t = lane & 15, g = lane >> 4;
@@ -779,7 +787,7 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
   }
   const Deal8 deal = deal8(A, all, some, n0);
   const int pairs = deal.pairs, side = deal.side, toll = deal.toll;
-  int64_t cur = (int64_t)blockIdx.x * deal.share;
+  int64_t cur = (int64_t)group * deal.share;
   int64_t end = cur + deal.share;
   int64_t u = 0, base = 0;   // base: where the pair begins that `cur` lies in
   for (;;) {
@@ -1038,7 +1046,7 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
           acc[1] += *reinterpret_cast<const float4v*>(rows + (((chunk + 16) ^ row) << 4)) * f;
         }
         const int hd = pair * side + h;
-        const int64_t place = part_place(side, blockIdx.x, j0 == 0, h, row);
+        const int64_t place = part_place(side, group, j0 == 0, h, row);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           if (whole)
@@ -1050,7 +1058,7 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
       }
     }
     if (j0 == 0 && (int)threadIdx.x < side) {   // the pair's first run says where the others are
-      Left8 left = {(int)blockIdx.x, 0, side, (int)threadIdx.x};
+      Left8 left = {group, 0, side, (int)threadIdx.x};
       if (!whole) left.n = 1 + (int)quotient(nt - j1 + deal.share - 1, deal.share);
       part_left(A)[u * C.KVH + pair * side + threadIdx.x] = left;
     }
@@ -1075,10 +1083,10 @@ __global__ __launch_bounds__(kThreadsA, 2) void attn8_kernel(Attn8Args A) {
 // enough pairs to fill the GPU, and so few parts of each), or for one row, whose
 // parts it reads eight at a time.
 template <int E, bool MANY>
-__global__ __launch_bounds__(256) void join8_kernel(Attn8Args A) {
+__device__ __forceinline__ void narrow_join(const Attn8Args& A, uint32_t block) {
   const Cache8& C = A.C;
   const int grp = threadIdx.x >> 5, chunk = threadIdx.x & 31;
-  const uint32_t id = MANY ? blockIdx.x : blockIdx.x / (uint32_t)kRowsA;
+  const uint32_t id = MANY ? block : block / (uint32_t)kRowsA;
   const int head = (int)(id % (uint32_t)C.KVH);
   const int64_t u = id / (uint32_t)C.KVH;
   const Left8 left = part_left(A)[id];
@@ -1119,7 +1127,7 @@ __global__ __launch_bounds__(256) void join8_kernel(Attn8Args A) {
       store_out<E>(A, out_row(A, U, head, row) + 4 * chunk, acc, L);
     }
   } else {
-    const int row = (int)(blockIdx.x % (uint32_t)kRowsA);
+    const int row = (int)(block % (uint32_t)kRowsA);
     if (row >= U.rows) return;
     float M = kMaxSentinel, L = 0.f;
     float4v acc = {0.f, 0.f, 0.f, 0.f};
@@ -1216,6 +1224,13 @@ constexpr int kTileBytesB = kTileB * kRowB;         // of K or of V
 constexpr int kChunkB = 64;                         // tiles whose Meta8 are held at once
 constexpr int kSegs = kTileB / 16;                  // 16-token segments of a tile
 static_assert(kChunkB * kSegs == kThreadsB, "a thread a segment");
+static_assert(kThreadsA == kThreadsB, "one launch for both kernels");
+
+// The workspace behind the narrow kernel's: partial rows, and their sums.
+__device__ __forceinline__ float* wide_rows(const Attn8Args& A) { return A.part + A.wide_at; }
+__device__ __forceinline__ float* wide_sums(const Attn8Args& A) {
+  return wide_rows(A) + A.units * A.C.KVH * A.splits * kRowsB * kHeadDim;
+}
 
 // The tiles of split s of a pair.
 __device__ __forceinline__ void split_tiles(const Attn8Args& A, int nt, int s, int& j0, int& j1) {
@@ -1224,21 +1239,29 @@ __device__ __forceinline__ void split_tiles(const Attn8Args& A, int nt, int s, i
   j1 = min(j0 + per, nt);
 }
 
-template <int CODE, int E>
-__global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
-  __shared__ __align__(16) char ks[2][kTileBytesB], vs[2][kTileBytesB];
-  __shared__ Meta8 metas[kThreadsB];
-  __shared__ __align__(16) uint2 places[kThreadsB];   // a segment's bytes from the KV head's first, or (y < 0) none
+struct WideLds {
+  char k[2][kTileBytesB], v[2][kTileBytesB];
+  Meta8 metas[kThreadsB];
+  uint2 places[kThreadsB];   // a segment's bytes from the KV head's first, or (y < 0) none
   // e4m3, tiles that not every row sees whole: whether V tile i & 3 has a NaN,
   // and which channels of each token
-  __shared__ int nan_seen[4];
-  __shared__ __align__(16) uint8_t nan_map[2][kTileB][kHeadDim / 8];
+  uint8_t nan_map[2][kTileB][kHeadDim / 8];
+  int nan_seen[4];
+};
+
+template <int CODE, int E>
+__device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideLds& L8) {
+  auto& ks = L8.k;
+  auto& vs = L8.v;
+  auto& metas = L8.metas;
+  auto& places = L8.places;
+  auto& nan_seen = L8.nan_seen;
+  auto& nan_map = L8.nan_map;
   const Cache8& C = A.C;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
   // KV heads fastest (they go to different XCDs' caches), then splits; the last
   // rows of a sequence, which have the most tiles, first
-  uint32_t id = blockIdx.x;
   const int head = (int)(id % (uint32_t)C.KVH);
   id /= (uint32_t)C.KVH;
   const int split = (int)(id % (uint32_t)A.splits);
@@ -1283,11 +1306,12 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
   for (int i0 = j0; i0 < j1; i0 += kChunkB) {
     const int cnt = min(j1 - i0, kChunkB);
     __syncthreads();
+    // a thread a segment: its place, for the loads, and then what its tokens weigh by
+    const int my_i = threadIdx.x / kSegs;
+    const int my_at = kTileB * U.tile(i0 + min(my_i, cnt - 1)) + 16 * (threadIdx.x % kSegs);
+    const int my_page = page8(C, entry8(C, U.s.b, my_at, my_i < cnt && my_at < hi));
     {
-      const int i = threadIdx.x / kSegs;
-      const int tok = kTileB * U.tile(i0 + min(i, cnt - 1)) + 16 * (threadIdx.x % kSegs);
-      const int page = page8(C, entry8(C, U.s.b, tok, i < cnt && tok < hi));
-      metas[threadIdx.x] = meta8(A, page, scales8(C, page, head, tok));
+      const int page = my_page, tok = my_at;
       const uint64_t off = page >= 0 ? (uint64_t)row_offset(C, page, 0, tok) : ~0ull;
       places[threadIdx.x] = uint2{(uint32_t)off, (uint32_t)(off >> 32)};
       if (threadIdx.x < 4) nan_seen[threadIdx.x] = 0;
@@ -1342,6 +1366,7 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
 
 #pragma unroll
     for (int g = 0; g < kSegs; ++g) load(0, g);
+    metas[threadIdx.x] = meta8(A, my_page, scales8(C, my_page, head, my_at));
     mend(0);
 #pragma unroll
     for (int g = 0; g < kSegs; ++g) {
@@ -1473,21 +1498,20 @@ __global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
       if (whole)
         store_out<E>(A, c, v, l);
       else
-        *reinterpret_cast<float4v*>(A.part + c) = v;
+        *reinterpret_cast<float4v*>(wide_rows(A) + c) = v;
     }
   if (!whole && hf == 0) {
-    float* ml = A.part + A.units * C.KVH * A.splits * kRowsB * kHeadDim;
-    ml[at / kHeadDim] = m;
-    ml[A.units * C.KVH * A.splits * kRowsB + at / kHeadDim] = l;
+    *reinterpret_cast<float2v*>(wide_sums(A) + 2 * (at / kHeadDim)) = float2v{m, l};
   }
 }
 
-// Joins the splits of the wide kernel's rows, 32 threads a row.
+// Joins the splits of the wide kernel's rows, 32 threads a row, eight splits on
+// their way.
 template <int E>
-__global__ __launch_bounds__(256) void wide_join8_kernel(Attn8Args A) {
+__device__ __forceinline__ void wide_join(const Attn8Args& A, uint32_t block) {
   const Cache8& C = A.C;
-  const int64_t pair = blockIdx.x / (kRowsB / 8);
-  const int row = 8 * (int)(blockIdx.x % (kRowsB / 8)) + (threadIdx.x >> 5), chunk = threadIdx.x & 31;
+  const int64_t pair = block / (kRowsB / 8);
+  const int row = 8 * (int)(block % (kRowsB / 8)) + (threadIdx.x >> 5), chunk = threadIdx.x & 31;
   const int64_t u = pair / C.KVH;
   const int head = (int)(pair - u * C.KVH);
   const Unit8 U = unit_b(A, u);
@@ -1495,23 +1519,76 @@ __global__ __launch_bounds__(256) void wide_join8_kernel(Attn8Args A) {
   int j0, j1;
   split_tiles(A, nt, 0, j0, j1);
   if (row >= U.rows || j1 == nt) return;
-  const int64_t rows = A.units * C.KVH * A.splits * kRowsB;
-  const float* pm = A.part + rows * kHeadDim;
-  const float* pl = pm + rows;
   const int64_t first = pair * A.splits * kRowsB + row;
   const int splits = (nt + j1 - 1) / j1;
-  float M = -INFINITY;
-  for (int s = 0; s < splits; ++s) M = fmaxf(M, pm[first + s * kRowsB]);
-  const float ref = M == -INFINITY ? 0.f : M;
+  const float2v* sums = reinterpret_cast<const float2v*>(wide_sums(A));
+  float M = -INFINITY, L = 0.f;
   float4v acc = {0.f, 0.f, 0.f, 0.f};
-  float L = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const int64_t p = first + s * kRowsB;
-    const float f = __builtin_amdgcn_exp2f(pm[p] - ref);
-    L = __builtin_fmaf(pl[p], f, L);
-    acc += *reinterpret_cast<const float4v*>(A.part + p * kHeadDim + 4 * chunk) * f;
+  for (int s0 = 0; s0 < splits; s0 += 8) {
+    float2v ml[8];
+    float4v a[8];
+    float top = M;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t p = first + (int64_t)min(s0 + k, splits - 1) * kRowsB;
+      ml[k] = sums[p];
+      a[k] = *reinterpret_cast<const float4v*>(wide_rows(A) + p * kHeadDim + 4 * chunk);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k][0]);
+    const float ref = top == -INFINITY ? 0.f : top;   // (a row that saw nothing yet)
+    const float again = __builtin_amdgcn_exp2f(M - ref);
+    M = top;
+    acc = acc * again;
+    L *= again;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (s0 + k < splits) {
+        const float f = __builtin_amdgcn_exp2f(ml[k][0] - ref);
+        acc += a[k] * f;
+        L = __builtin_fmaf(ml[k][1], f, L);
+      }
   }
   store_out<E>(A, out_row(A, U, head, row) + 4 * chunk, acc, L);
+}
+
+// ---- launches ----
+//
+// A call is two launches: the attention of its narrow sequences, of its wide ones
+// or of both at once (the wide ones' workgroups first, which have the most to do),
+// and the join of what was left in parts.
+
+template <int CODE, int E>
+__global__ __launch_bounds__(kThreadsA, 2) void narrow8_kernel(Attn8Args A) {
+  __shared__ __align__(16) NarrowLds lds;
+  narrow_part<CODE, E>(A, (int)blockIdx.x, lds);
+}
+
+template <int CODE, int E>
+__global__ __launch_bounds__(kThreadsB, 2) void wide8_kernel(Attn8Args A) {
+  __shared__ __align__(16) WideLds lds;
+  wide_part<CODE, E>(A, blockIdx.x, lds);
+}
+
+template <int CODE, int E>
+__global__ __launch_bounds__(kThreadsB, 2) void both8_kernel(Attn8Args A) {
+  __shared__ __align__(16) union {
+    NarrowLds narrow;
+    WideLds wide;
+  } lds;
+  const uint32_t wide = gridDim.x - A.groups;
+  if (blockIdx.x < wide)
+    wide_part<CODE, E>(A, blockIdx.x, lds.wide);
+  else
+    narrow_part<CODE, E>(A, (int)(blockIdx.x - wide), lds.narrow);
+}
+
+template <int E, bool MANY>
+__global__ __launch_bounds__(256) void join8_kernel(Attn8Args A) {
+  if (blockIdx.x < A.wide_blocks)
+    wide_join<E>(A, blockIdx.x);
+  else
+    narrow_join<E, MANY>(A, blockIdx.x - A.wide_blocks);
 }
 
 // ---------------------------------------------------------------------------
@@ -1632,28 +1709,27 @@ size_t wide_bytes(int64_t units, int32_t KVH, int splits) {
 
 size_t attn_bytes(bool offsets, int64_t B, int64_t T, int32_t G, int32_t KVH, int64_t max_len) {
   const int64_t units = wide_units(offsets, B, T, G);
-  return std::max(narrow_bytes(narrow_groups(B, KVH, G, max_len), narrow_side(KVH), B * KVH),
-                  wide_bytes(units, KVH, wide_splits(units, KVH, max_len)));
+  return narrow_bytes(narrow_groups(B, KVH, G, max_len), narrow_side(KVH), B * KVH) +
+         wide_bytes(units, KVH, wide_splits(units, KVH, max_len));
 }
 
 template <int CODE, int E>
 int launch_attn8(Attn8Args A, hipStream_t stream) {
-  // one after the other: both kernels' partial rows go to the same workspace
-  if (A.groups > 0) {
-    attn8_kernel<CODE, E><<<dim3((unsigned)A.groups), dim3(kThreadsA), 0, stream>>>(A);
-    const int64_t heads = A.C.B * A.C.KVH;
-    if (heads / A.side >= kManyPairs)
-      join8_kernel<E, true><<<dim3((unsigned)heads), dim3(256), 0, stream>>>(A);
-    else
-      join8_kernel<E, false><<<dim3((unsigned)(heads * kRowsA)), dim3(256), 0, stream>>>(A);
-    const int rc = launch_status();
-    if (rc) return rc;
-  }
-  if (A.units > 0) {
-    wide8_kernel<CODE, E><<<dim3((unsigned)(A.units * A.C.KVH * A.splits)), dim3(kThreadsB), 0, stream>>>(A);
-    if (A.splits > 1)
-      wide_join8_kernel<E><<<dim3((unsigned)(A.units * A.C.KVH * (kRowsB / 8))), dim3(256), 0, stream>>>(A);
-  }
+  const unsigned wide = (unsigned)(A.units * A.C.KVH * A.splits);
+  if (A.groups == 0)
+    wide8_kernel<CODE, E><<<dim3(wide), dim3(kThreadsB), 0, stream>>>(A);
+  else if (wide == 0)
+    narrow8_kernel<CODE, E><<<dim3((unsigned)A.groups), dim3(kThreadsA), 0, stream>>>(A);
+  else
+    both8_kernel<CODE, E><<<dim3(wide + A.groups), dim3(kThreadsB), 0, stream>>>(A);
+  const int rc = launch_status();
+  if (rc) return rc;
+  A.wide_blocks = A.splits > 1 ? (unsigned)(A.units * A.C.KVH * (kRowsB / 8)) : 0;
+  const int64_t heads = A.groups ? A.C.B * A.C.KVH : 0;
+  if (heads / A.side >= kManyPairs)
+    join8_kernel<E, true><<<dim3(A.wide_blocks + (unsigned)heads), dim3(256), 0, stream>>>(A);
+  else if (A.wide_blocks + heads > 0)
+    join8_kernel<E, false><<<dim3(A.wide_blocks + (unsigned)(heads * kRowsA)), dim3(256), 0, stream>>>(A);
   return launch_status();
 }
 
@@ -1725,12 +1801,13 @@ int kvdec_paged8_attention(const kvdec_paged8_cache* cache, const void* q, void*
   A.side = narrow_side(A.C.KVH);
   A.units = wide_units(offsets, B, T, A.G);
   A.splits = wide_splits(A.units, A.C.KVH, A.C.max_len);
-  if (B * A.C.KVH * kRowsA > 0x7fffffff || A.units * A.C.KVH * std::max(A.splits, kRowsB / 8) > 0x7fffffff)
+  if (B * A.C.KVH * kRowsA + A.units * A.C.KVH * std::max(A.splits, kRowsB / 8) + A.groups > 0x7fffffff)
     return KVDEC_E_SHAPE;
   if (!ws || !on16(ws) || ws_bytes < attn_bytes(offsets, B, T, A.G, A.C.KVH, A.C.max_len)) return KVDEC_E_WORKSPACE;
   A.q = q;
   A.o = o;
   A.part = static_cast<float*>(ws);
+  A.wide_at = (int64_t)(narrow_bytes(A.groups, narrow_side(A.C.KVH), B * A.C.KVH) / sizeof(float));
   A.q_tok = q_token_stride;
   A.q_head = q_head_stride;
   A.H = H;
