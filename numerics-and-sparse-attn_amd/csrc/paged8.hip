@@ -506,8 +506,9 @@ struct Attn8Args {
   int64_t q_tok, q_head;      // in elements
   int64_t units;
   int32_t G, H, window, sink;
-  int32_t groups;             // narrow: workgroups,
-  int32_t side;               // and KV heads that one may read side by side (1, 2 or 4)
+  int32_t groups;             // narrow: workgroups (a power of two),
+  int32_t side, pairs;        // KV heads that one may read side by side (1, 2 or 4), and KVH / side
+  uint32_t inv_g;             // 65536 / G rounded up: row / G of a narrow row is row * inv_g >> 16
   int32_t splits;             // wide: workgroups a pair,
   uint32_t wide_blocks;       // and those of the join
   float scale_log2;
@@ -524,15 +525,15 @@ struct Unit8 {
 };
 
 template <int TILE>
-__device__ __forceinline__ void unit_tiles(const Attn8Args& A, Unit8& U) {
+__device__ __forceinline__ void unit_tiles(const Attn8Args& A, Unit8& U, int pos0, int pos1) {
   U.ts = U.tw = U.te = 0;
   U.pos0 = U.pos1 = -1;
   if (U.rows <= 0) {
     U.rows = 0;
     return;
   }
-  U.pos0 = U.s.len - U.s.n + U.row0 / A.G;
-  U.pos1 = U.s.len - U.s.n + (U.row0 + U.rows - 1) / A.G;
+  U.pos0 = pos0;
+  U.pos1 = pos1;
   if (U.pos1 < 0) return;
   U.te = U.pos1 / TILE + 1;
   if (A.window > 0) {
@@ -542,15 +543,15 @@ __device__ __forceinline__ void unit_tiles(const Attn8Args& A, Unit8& U) {
 }
 
 // The narrow kernel's unit: a sequence, if its rows fit.
-__device__ __forceinline__ Unit8 unit_a(const Attn8Args& A, int64_t b) {
+__device__ __forceinline__ Unit8 unit_a(const Attn8Args& A, const Seq8& s) {
   Unit8 U;
-  U.s = seq8(A.C, b);
-  const int64_t rows = (int64_t)U.s.n * A.G;
+  U.s = s;
   U.row0 = 0;
-  U.rows = rows <= kRowsA ? (int)rows : 0;
-  unit_tiles<kTile>(A, U);
+  U.rows = (int64_t)s.n * A.G <= kRowsA ? s.n * A.G : 0;
+  unit_tiles<kTile>(A, U, s.len - s.n, s.len - 1);
   return U;
 }
+__device__ __forceinline__ Unit8 unit_a(const Attn8Args& A, int64_t b) { return unit_a(A, seq8(A.C, b)); }
 
 // The same by halving, on scalars alone (the wide kernel has no registers for the
 // search above: 15% of its time).
@@ -583,7 +584,8 @@ __device__ __forceinline__ Unit8 unit_b(const Attn8Args& A, int64_t u) {
   const int64_t rows = (int64_t)U.s.n * A.G, row0 = max(u - first, (int64_t)0) * kRowsB;
   U.row0 = (int)min(row0, rows);
   U.rows = rows > kRowsA || U.s.b == C.B ? (int)min(rows - U.row0, (int64_t)kRowsB) : 0;
-  unit_tiles<kTileB>(A, U);
+  const int p0 = U.s.len - U.s.n;
+  unit_tiles<kTileB>(A, U, p0 + U.row0 / A.G, p0 + (U.row0 + U.rows - 1) / A.G);
   return U;
 }
 
@@ -660,13 +662,28 @@ __device__ __forceinline__ uint32_t upto_lane(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t last_lane(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
 
-// Tiles of one KV head of sequence u0 + lane.
+// Sequence v (none past the last), and its tiles of one KV head.
+__device__ __forceinline__ Seq8 seq_a(const Attn8Args& A, int64_t v) {
+  return v < A.C.B ? seq8(A.C, v) : Seq8{(int)v, 0, 0, 0};
+}
 __device__ __forceinline__ uint32_t tiles_a(const Attn8Args& A, int64_t v) {
-  return v < A.C.B ? (uint32_t)unit_a(A, v).tiles() : 0u;
+  return (uint32_t)unit_a(A, seq_a(A, v)).tiles();
 }
 
+// a / b rounded up, b > 0; small ones by a reciprocal, put right by one.
+__device__ __forceinline__ uint32_t up(uint32_t a, uint32_t b) {
+  if ((a | b) >> 21) return a / b + (a % b != 0);
+  uint32_t q = (uint32_t)((float)a * __builtin_amdgcn_rcpf((float)b));
+  const int left = (int)(a - q * b);
+  q = left < 0 ? q - 1 : left >= (int)b ? q + 1 : q;
+  return q + (q * b != a);
+}
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {   // of numbers >= 0
   return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+// At least a / b, and little more.
+__device__ __forceinline__ int64_t about(int64_t a, int64_t b) {
+  return (int64_t)((float)a * __builtin_amdgcn_rcpf((float)b) * 1.0001f) + 1;
 }
 
 // How a launch's tiles are dealt (all: one KV head's, some: sequences with any).
@@ -687,7 +704,7 @@ struct Deal8 {
   // what a pair of n tiles takes of the runs' common line
   __device__ __forceinline__ int64_t length(uint32_t n) const {
     if (n == 0) return 0;
-    return alone ? (int64_t)((n + (uint32_t)share - 1) / (uint32_t)share) * share : (int64_t)n + toll;
+    return alone ? (int64_t)up(n, (uint32_t)share) * share : (int64_t)n + toll;
   }
 };
 constexpr int kLongRun = 16, kLeastRounds = 2;
@@ -698,25 +715,25 @@ __device__ __forceinline__ Deal8 deal8(const Attn8Args& A, int64_t all, int64_t 
   const bool lengthy = all * A.C.KVH >= (int64_t)kLongRun * kWavesA * A.groups;
   const bool far = lengthy && A.C.head_bytes < (int64_t)A.C.row_bytes;
   d.side = (crowd | far) ? A.side : 1;
-  d.pairs = A.C.KVH / d.side;
-  const int phases = kWavesA / d.side;
+  d.pairs = (crowd | far) ? A.pairs : A.C.KVH;
+  const int phases = (crowd | far) ? kWavesA / A.side : kWavesA;
   const int64_t count = some * d.pairs;
   d.alone = !lengthy & (2 * count <= A.groups);
   d.toll = 2 * count > A.groups ? 4 * phases : 0;
   // runs no shorter than a pair of few tiles, or two tiles for each wave of a head
-  const int64_t least = min(quotient(all + some - 1, max(some, (int64_t)1)), (int64_t)kLeastRounds * phases);
-  const int64_t even = max(quotient((all + some * d.toll) * d.pairs + A.groups - 1, A.groups), max(least, (int64_t)1));
+  const int64_t least = all <= (int64_t)kLeastRounds * phases * some ? about(all, max(some, (int64_t)1)) : kLeastRounds * phases;
+  const int64_t even = max(((all + some * d.toll) * d.pairs + A.groups - 1) >> __builtin_ctz(A.groups), least);
   d.share = even;
   if (d.alone) {
     // all / share parts and one a pair are enough workgroups for certain; with
     // 64 sequences at most, the least of some shares between that does
-    const int64_t sure = max(quotient(all * d.pairs + A.groups - count - 1, A.groups - count), even);
+    const int64_t sure = max(about(all * d.pairs, A.groups - count), even);
     d.share = sure;
-    if (A.C.B <= 64) {
+    if (A.C.B <= 64 && sure > even) {
 #pragma unroll
-      for (int k = 2; k >= 0; --k) {
-        const uint32_t t = (uint32_t)(even + (sure - even) * k / 3);
-        const uint32_t parts = last_lane(upto_lane((n + t - 1) / t));
+      for (int k = 1; k >= 0; --k) {
+        const uint32_t t = (uint32_t)(even + (k ? (sure - even) >> 1 : 0));
+        const uint32_t parts = last_lane(upto_lane(up(n, t)));
         if ((int64_t)parts * d.pairs <= A.groups) d.share = t;
       }
     }
@@ -773,7 +790,8 @@ __device__ __forceinline__ void narrow_part(const Attn8Args& A, int group, Narro
   char* slot = lds + wave * kSlotA;
 
   // this workgroup's run of tiles, and the sequence that it starts in
-  uint32_t n0 = tiles_a(A, lane);
+  Seq8 s0 = seq_a(A, lane);
+  uint32_t n0 = (uint32_t)unit_a(A, s0).tiles();
   int64_t all = last_lane(upto_lane(n0)), some = __builtin_popcountll(__ballot(n0 != 0));
   for (int64_t u0 = 64; u0 < C.B; u0 += 256) {   // four loads on their way
     uint32_t n = 0;
@@ -790,6 +808,7 @@ __device__ __forceinline__ void narrow_part(const Attn8Args& A, int group, Narro
   int64_t cur = (int64_t)group * deal.share;
   int64_t end = cur + deal.share;
   int64_t u = 0, base = 0;   // base: where the pair begins that `cur` lies in
+  Unit8 U;
   for (;;) {
     const uint32_t mine = (uint32_t)deal.length(n0), upto = upto_lane(mine);
     const uint64_t past = __ballot(base + (int64_t)upto * pairs > cur);
@@ -797,14 +816,16 @@ __device__ __forceinline__ void narrow_part(const Attn8Args& A, int group, Narro
       const int first = __builtin_ctzll(past);
       base += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), first) * pairs;
       u += first;
+      U = unit_a(A, Seq8{(int)u, __builtin_amdgcn_readlane(s0.c0, first), __builtin_amdgcn_readlane(s0.n, first),
+                         __builtin_amdgcn_readlane(s0.len, first)});
       break;
     }
     base += (int64_t)last_lane(upto) * pairs;
     u += 64;
     if (u >= C.B) return;    // no run is left
-    n0 = tiles_a(A, u + lane);
+    s0 = seq_a(A, u + lane);
+    n0 = (uint32_t)unit_a(A, s0).tiles();
   }
-  Unit8 U = unit_a(A, u);
   int64_t length = deal.length(U.tiles());
   int pair = (int)quotient(cur - base, length);
   base += (int64_t)pair * length;
@@ -818,8 +839,7 @@ __device__ __forceinline__ void narrow_part(const Attn8Args& A, int group, Narro
     const int head = pair * side + wave % side;
 
     // this lane's query row
-    const int my_row = U.row0 + t;
-    const int my_tok = my_row / A.G, my_head = my_row - my_tok * A.G;
+    const int my_tok = (int)((uint32_t)t * A.inv_g >> 16), my_head = t - my_tok * A.G;
     const int pos = t < U.rows ? U.s.len - U.s.n + my_tok : -1;
     half8 qB[4];
 #pragma unroll
@@ -1089,7 +1109,12 @@ __device__ __forceinline__ void narrow_join(const Attn8Args& A, uint32_t block) 
   const uint32_t id = MANY ? block : block / (uint32_t)kRowsA;
   const int head = (int)(id % (uint32_t)C.KVH);
   const int64_t u = id / (uint32_t)C.KVH;
-  const Left8 left = part_left(A)[id];
+  Left8 left = part_left(A)[id];
+  // (inside the workspace whatever it holds)
+  left.side = left.side == A.side ? A.side : 1;
+  left.h = left.h & (left.side - 1);
+  left.first = min(max(left.first, 0), A.groups - 1);
+  left.n = min(max(left.n, 0), A.groups - left.first);
   const Unit8 U = unit_a(A, u);
   const bool none = U.tiles() == 0;        // (then nothing is said of its rows)
   if (!none && left.n == 0) return;
@@ -1683,7 +1708,9 @@ int launch_read(const Read8Args& A, int dtype, hipStream_t stream) {
 int narrow_groups(int64_t B, int32_t KVH, int32_t G, int64_t max_len) {
   if (G > kRowsA) return 0;
   const int64_t tiles = B * KVH * ((max_len + kTile - 1) / kTile);
-  return (int)std::min<int64_t>(kGroupsA, std::max<int64_t>(1, (tiles + kWavesA - 1) / kWavesA));
+  int groups = 1;
+  while (groups < kGroupsA && (int64_t)groups * kWavesA < tiles) groups *= 2;
+  return groups;
 }
 size_t narrow_bytes(int groups, int side, int64_t heads) {
   return groups ? (size_t)part_rows(groups, side) * (kHeadDim + 2) * sizeof(float) + (size_t)heads * sizeof(Left8) : 0;
@@ -1799,6 +1826,8 @@ int kvdec_paged8_attention(const kvdec_paged8_cache* cache, const void* q, void*
   const bool offsets = cu_seqlens != nullptr;
   A.groups = narrow_groups(B, A.C.KVH, A.G, A.C.max_len);
   A.side = narrow_side(A.C.KVH);
+  A.pairs = A.C.KVH / A.side;
+  A.inv_g = (uint32_t)((65536 + A.G - 1) / A.G);
   A.units = wide_units(offsets, B, T, A.G);
   A.splits = wide_splits(A.units, A.C.KVH, A.C.max_len);
   if (B * A.C.KVH * kRowsA + A.units * A.C.KVH * std::max(A.splits, kRowsB / 8) + A.groups > 0x7fffffff)
