@@ -34,8 +34,8 @@ extern "C" {
  *   block_table : [B, max_blocks] int32; an entry outside [0, num_pages) is no
  *     page: its tokens are not written, read as zeros, and weigh in attention
  *     as keys and values of zero
- *   seq_lens : [B] int32, the tokens of each sequence with its new ones;
- *     clamped into [0, max_blocks * page_size]
+ *   seq_lens : [B] int32, the tokens of each sequence with its new ones (below
+ *     0: 0).  Positions past the table have no page; attention has no keys there
  *   page_size : a power of two, 16 or more; block_size 16, 32, 64 or 128 and
  *     at most page_size; max_blocks * page_size < 2^30
  */

@@ -58,7 +58,7 @@ __device__ __forceinline__ Seq8 seq8(const Cache8& C, int64_t b) {
     s.c0 = offset8(C, b);
     s.n = (b < C.B ? offset8(C, b + 1) : (int)C.T) - s.c0;
   }
-  s.len = b < C.B ? min(max((int)((cint32*)C.lens)[b], 0), C.max_len) : 0;
+  s.len = b < C.B ? max((int)((cint32*)C.lens)[b], 0) : 0;
   return s;
 }
 
@@ -87,7 +87,7 @@ __device__ __forceinline__ Found8 find8(const Cache8& C, int64_t u, int lane, Fi
   if (lane < n) {
     c0 = offset8(C, s);
     c1 = s < C.B ? offset8(C, s + 1) : (int)C.T;
-    if (s < C.B) len = min(max(((const int32_t*)C.lens)[s], 0), C.max_len);
+    if (s < C.B) len = max(((const int32_t*)C.lens)[s], 0);
   }
   const bool ok = lane < n && first(c0, s) <= u;
   const int at = __builtin_amdgcn_readfirstlane(max((int)__builtin_popcountll(__ballot(ok)), 1) - 1);
@@ -102,7 +102,7 @@ __device__ __forceinline__ Found8 find8(const Cache8& C, int64_t u, int lane, Fi
 
 // The tokens of unit u that lie in one block of one sequence: rows [r0, r1) of
 // the block that starts at position `start`, whose row r is token c + r of the
-// call.  page < 0: no page holds them (also positions below 0).
+// call.  page < 0: no page holds them (also positions below 0 and past the table).
 struct Run8 {
   int64_t start, c;
   int r0, r1;
@@ -126,7 +126,7 @@ __device__ __forceinline__ Run8 run8(const Cache8& C, int64_t u, int lane) {
   r.r0 = (int)min(max(p0 - r.start, (int64_t)0), block);
   r.r1 = s.n > 0 ? (int)max(min((int64_t)s.len - r.start, block), (int64_t)0) : 0;
   r.page = -1;
-  if (r.r1 > r.r0 && r.start >= 0) {   // then start < len <= max_len
+  if (r.r1 > r.r0 && r.start >= 0 && r.start < C.max_len) {
     const int64_t id = ((cint32*)C.bt)[(int64_t)s.b * C.max_blocks + (r.start >> C.ps_log2)];
     if (id >= 0 && id < C.num_pages) r.page = id;
   }
@@ -515,10 +515,11 @@ struct Attn8Args {
 };
 
 // A unit: query rows [row0, row0 + rows) of a sequence's n * G, at positions
-// pos0 .. pos1, and its tiles: [0, ts) of the sink and [tw, te).
+// pos0 .. pos1, whose keys end before hi, and its tiles: [0, ts) of the sink and
+// [tw, te).
 struct Unit8 {
   Seq8 s;
-  int row0, rows, pos0, pos1;
+  int row0, rows, pos0, pos1, hi;
   int ts, tw, te;
   __device__ __forceinline__ int tiles() const { return ts + te - tw; }
   __device__ __forceinline__ int tile(int j) const { return j < ts ? j : tw + j - ts; }
@@ -526,7 +527,7 @@ struct Unit8 {
 
 template <int TILE>
 __device__ __forceinline__ void unit_tiles(const Attn8Args& A, Unit8& U, int pos0, int pos1) {
-  U.ts = U.tw = U.te = 0;
+  U.ts = U.tw = U.te = U.hi = 0;
   U.pos0 = U.pos1 = -1;
   if (U.rows <= 0) {
     U.rows = 0;
@@ -535,7 +536,8 @@ __device__ __forceinline__ void unit_tiles(const Attn8Args& A, Unit8& U, int pos
   U.pos0 = pos0;
   U.pos1 = pos1;
   if (U.pos1 < 0) return;
-  U.te = U.pos1 / TILE + 1;
+  U.hi = min(U.pos1, A.C.max_len - 1) + 1;
+  U.te = (U.hi + TILE - 1) / TILE;
   if (A.window > 0) {
     U.ts = min((int)(((int64_t)A.sink + TILE - 1) / TILE), U.te);
     U.tw = min(max(U.ts, max(U.pos0 - A.window + 1, 0) / TILE), U.te);
@@ -589,14 +591,19 @@ __device__ __forceinline__ Unit8 unit_b(const Attn8Args& A, int64_t u) {
   return U;
 }
 
-// Where a token of a tile stands against a row's position.
-__device__ __forceinline__ bool sees(int p, int pos, int window, int sink) {
-  return (p <= pos) & ((window <= 0) | (p < sink) | (p > pos - window));
+// The positions that a query row sees: up to `upto`, and before `sink` or from
+// `from` on.
+struct Sight8 {
+  int upto, from, sink;
+  __device__ __forceinline__ bool sees(int p) const { return (p <= upto) & ((p < sink) | (p >= from)); }
+};
+__device__ __forceinline__ Sight8 sight8(const Attn8Args& A, const Unit8& U, int pos) {
+  return A.window > 0 ? Sight8{min(pos, U.hi - 1), pos - A.window + 1, A.sink} : Sight8{min(pos, U.hi - 1), 0, 0};
 }
 
 // Every token of [tok, tok + n) is seen by every row of the unit.
 __device__ __forceinline__ bool all_seen(const Attn8Args& A, const Unit8& U, int tok, int n) {
-  return (tok + n - 1 <= U.pos0) & ((A.window <= 0) | (tok + n <= A.sink) | (tok > U.pos1 - A.window));
+  return (tok + n - 1 <= min(U.pos0, U.hi - 1)) & ((A.window <= 0) | (tok + n <= A.sink) | (tok > U.pos1 - A.window));
 }
 
 // What a token of the pair's rows weighs by: kf turns q . k into x, lv is
@@ -841,7 +848,7 @@ __device__ __forceinline__ void narrow_part(const Attn8Args& A, int group, Narro
 
     // this lane's query row
     const int my_tok = (int)((uint32_t)t * A.inv_g >> 16), my_head = t - my_tok * A.G;
-    const int pos = t < U.rows ? U.s.len - U.s.n + my_tok : -1;
+    const Sight8 sight = sight8(A, U, t < U.rows ? U.s.len - U.s.n + my_tok : -1);
     half8 qB[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -859,7 +866,7 @@ __device__ __forceinline__ void narrow_part(const Attn8Args& A, int group, Narro
     st.m = kMaxSentinel;
     st.l = 0.f;
 
-    const int hi = U.pos1 + 1, lo = A.window > 0 ? max(U.pos0 - A.window + 1, 0) : 0;
+    const int hi = U.hi, lo = A.window > 0 ? max(U.pos0 - A.window + 1, 0) : 0;
     const int sink = A.window > 0 ? A.sink : 0;
     const char* kbase = C.k + head * C.head_bytes;
     const char* vbase = C.v + head * C.head_bytes;
@@ -958,7 +965,7 @@ __device__ __forceinline__ void narrow_part(const Attn8Args& A, int group, Narro
         if (!full) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const bool ok = sees(tok + tau(g, j), pos, A.window, sink);
+            const bool ok = sight.sees(tok + tau(g, j));
             seen |= (uint32_t)ok << j;
             x[j] = ok ? x[j] : -INFINITY;
           }
@@ -1303,7 +1310,7 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
   const int my_row = 32 * wave + n;
   const int my_tok = (U.row0 + my_row) / A.G, my_head = U.row0 + my_row - my_tok * A.G;
   const bool mine = my_row < U.rows;
-  const int pos = mine ? U.s.len - U.s.n + my_tok : -1;
+  const Sight8 sight = sight8(A, U, mine ? U.s.len - U.s.n + my_tok : -1);
   u32x4 qB[8];
 #pragma unroll
   for (int s = 0; s < 8; ++s) {
@@ -1319,7 +1326,7 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
     for (int r = 0; r < 16; ++r) O[cb][r] = 0.f;
   float m = -INFINITY, l = 0.f;   // no token seen yet; the lane's share of the sum
 
-  const int hi = U.pos1 + 1, lo = A.window > 0 ? max(U.pos0 - A.window + 1, 0) : 0;
+  const int hi = U.hi, lo = A.window > 0 ? max(U.pos0 - A.window + 1, 0) : 0;
   const int sink = A.window > 0 ? A.sink : 0;
   const char* kbase = C.k + head * C.head_bytes;
   const char* vbase = C.v + head * C.head_bytes;
@@ -1449,7 +1456,7 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const int p = tok + 32 * b + 8 * (r >> 2) + 4 * hf + (r & 3);
-              S[b][r] = sees(p, pos, A.window, A.sink) ? S[b][r] : -INFINITY;
+              S[b][r] = sight.sees(p) ? S[b][r] : -INFINITY;
             }
         }
 #pragma unroll
@@ -1498,7 +1505,7 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
         if (nans) {   // and reaches the rows that do
           u32x4 hit = {0u, 0u, 0u, 0u};   // this row's channels
           for (int p = 0; p < kTileB; ++p)
-            if (sees(tok + p, pos, A.window, A.sink)) hit |= *reinterpret_cast<const u32x4*>(nan_map[i & 1][p]);
+            if (sight.sees(tok + p)) hit |= *reinterpret_cast<const u32x4*>(nan_map[i & 1][p]);
 #pragma unroll
           for (int cb = 0; cb < 4; ++cb) {
             const uint32_t w = hit[cb] >> (4 * hf);

@@ -70,8 +70,8 @@ def _offsets(cu, B, T):
     return list(range(B + 1)) if cu is None else [0] + [min(max(int(c), 0), T) for c in cu[1:]]
 
 
-def _len(seq_lens, b, table, page_size):
-    return min(max(int(seq_lens[b]), 0), table.shape[1] * page_size)
+def _len(seq_lens, b):
+    return max(int(seq_lens[b]), 0)
 
 
 def _place(table, b, pos, page_size, num_pages):
@@ -93,7 +93,7 @@ def write(cache, k, v, table, seq_lens, cu, code, layout="NHD"):
         block = ps // scales.shape[2]
         for b in range(B):
             n = off[b + 1] - off[b]
-            length = _len(seq_lens, b, table, ps)
+            length = _len(seq_lens, b)
             p0 = length - n
             if n <= 0:
                 continue
@@ -155,7 +155,7 @@ def read(cache, table, seq_lens, cu, T, code, layout="NHD"):
         KVH, D = _heads_first(cache[name + "_pages"], layout).shape[1::2]
         out = np.zeros((T, KVH, D))
         for b in range(B):
-            length = _len(seq_lens, b, table, ps)
+            length = _len(seq_lens, b)
             n = off[b + 1] - off[b]
             if n > 0:
                 first = length - n
@@ -176,20 +176,21 @@ def attention(q, cache, table, seq_lens, cu, sm_scale, code, layout="NHD", windo
     off = _offsets(cu, B, T)
     o = np.zeros((T, H, D))
     for b in range(B):
-        length = _len(seq_lens, b, table, ps)
+        length = _len(seq_lens, b)
         n = off[b + 1] - off[b]
         if n <= 0 or length == 0:
             continue
-        kk = gather(cache, "k", table, b, 0, length, layout, code)
-        vv = gather(cache, "v", table, b, 0, length, layout, code)
+        held = min(length, table.shape[1] * ps)   # no keys past the table
+        kk = gather(cache, "k", table, b, 0, held, layout, code)
+        vv = gather(cache, "v", table, b, 0, held, layout, code)
         for i in range(n):
             pos = length - n + i
             if pos < 0:
                 continue
-            p = np.arange(pos + 1)
+            p = np.arange(min(pos + 1, held))
             if window is not None:
                 p = p[(p < sink) | (p > pos - window)]
-            for h in range(H):
+            for h in range(H if len(p) else 0):
                 x = kk[p, h // G] @ q[off[b] + i, h] * sm_scale
                 w = np.exp(x - np.max(x)) if not np.isnan(x).any() else np.full_like(x, np.nan)
                 o[off[b] + i, h] = w @ vv[p, h // G] / w.sum()

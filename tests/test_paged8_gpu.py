@@ -422,6 +422,30 @@ def test_masked_nan_stays_out(code, window, device):
     check_out(o, ref, "fp16", vmax_of(c, code), single=True)
 
 
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("window", [None, 30])
+def test_attend_past_the_table(many, window, device):
+    """Lengths past the block table, below 0 and more new tokens than length: keys
+    are the table's; bad entries are keys and values of zero."""
+    from paged8_kernel import paged8_attention
+    rng = np.random.default_rng(57)
+    H, KVH, ps = 4, 2, 16
+    lens = [70, 48, 1000, 2**31 - 1, -5, 20, 90]
+    new = [30, 1, 20, 40, 3, 25, 70] if many else [1] * 7
+    c = make_cache(rng, 24, KVH, ps, 16, "int8", "NHD")
+    table = rng.permutation(21).reshape(7, 3).astype(np.int32)
+    table[1, 1], table[5, 0], table[6, 2] = -1, 24, 2**31 - 1
+    cu = np.cumsum([0] + new) if many else None
+    q = torch.from_numpy(rng.standard_normal((sum(new), H, D)).astype(np.float32)).half()
+    sink = 5 if window else 0
+    ref = O.attention(q.double().numpy(), c, table, lens, cu, SCALE, "int8", window=window, sink=sink)
+    say(f"past the table, many {many} window {window}")
+    o = paged8_attention(q.to(device), *put(c, "int8", device), i32(table, device), i32(lens, device), i32(cu, device),
+                         window=window, sink=sink)
+    torch.cuda.synchronize()
+    check_out(o, ref, "fp16", vmax_of(c, "int8"), single=many)
+
+
 def test_attend_many_sequences(device):
     """More sequences than a wave has lanes, most of them short or empty."""
     from paged8_kernel import paged8_attention
