@@ -495,7 +495,8 @@ static_assert(kRowsA * kHeadDim * 4 <= kSlotA, "a wave's partial rows fit its sl
 constexpr int kRowsB = 128;                         // query rows of a workgroup, 32 a wave
 constexpr int kThreadsB = 256;
 constexpr int kTileB = 64;                          // tokens of its tiles
-constexpr int kPairsB = 512;                        // workgroups that fill the GPU
+constexpr int kPairsB = 512;                        // workgroups that fill the GPU,
+constexpr int kJoinsB = 1024;                       // and of a join
 
 struct Attn8Args {
   Cache8 C;
@@ -509,8 +510,9 @@ struct Attn8Args {
   int32_t groups;             // narrow: workgroups (a power of two),
   int32_t side, pairs;        // KV heads that one may read side by side (1, 2 or 4), and KVH / side
   uint32_t inv_g;             // 65536 / G rounded up: row / G of a narrow row is row * inv_g >> 16
-  int32_t splits;             // wide: workgroups a pair,
-  uint32_t wide_blocks;       // and those of the join
+  int32_t slots, few;         // wide: workgroups a KV head that the units are dealt to, and those that
+                              // fill the GPU; slots = 0: one a unit
+  uint32_t wide_blocks, passes;   // the join's workgroups for them, and the rows of each, by 8
   float scale_log2;
 };
 
@@ -568,27 +570,30 @@ __device__ __forceinline__ Found8 find8_scalar(const Cache8& C, int64_t u, First
   return Found8{s, first(s.c0, lo)};
 }
 
-// The wide kernel's unit u: kRowsB rows of a sequence of more than kRowsA, or of
-// the rows past the last sequence (which attend to nothing).
-__device__ __forceinline__ Unit8 unit_b(const Attn8Args& A, int64_t u) {
-  const Cache8& C = A.C;
+// The wide kernel's units are kRowsB rows of a sequence of more than kRowsA, or
+// of the rows past the last sequence (which attend to nothing).
+__device__ __forceinline__ int64_t rows_b(const Attn8Args& A, const Seq8& s) {
+  const int64_t rows = (int64_t)s.n * A.G;
+  return rows > kRowsA || s.b == A.C.B ? rows : 0;
+}
+__device__ __forceinline__ Unit8 unit_of(const Attn8Args& A, const Seq8& s, int64_t row0) {
   Unit8 U;
-  int64_t first;
-  if (C.cu == nullptr) {
-    const int per = (A.G + kRowsB - 1) / kRowsB;
-    first = u / per * per;
-    U.s = seq8(C, u / per);
-  } else {
-    const Found8 f = find8_scalar(C, u, [&](int c0, int64_t b) { return (int64_t)c0 * A.G / kRowsB + b; });
-    U.s = f.s;
-    first = f.first;
-  }
-  const int64_t rows = (int64_t)U.s.n * A.G, row0 = max(u - first, (int64_t)0) * kRowsB;
+  U.s = s;
+  const int64_t rows = rows_b(A, s);
   U.row0 = (int)min(row0, rows);
-  U.rows = rows > kRowsA || U.s.b == C.B ? (int)min(rows - U.row0, (int64_t)kRowsB) : 0;
-  const int p0 = U.s.len - U.s.n;
+  U.rows = (int)min(rows - U.row0, (int64_t)kRowsB);
+  const int p0 = s.len - s.n;
   unit_tiles<kTileB>(A, U, p0 + U.row0 / A.G, p0 + (U.row0 + U.rows - 1) / A.G);
   return U;
+}
+__device__ __forceinline__ Unit8 unit_b(const Attn8Args& A, int64_t u) {
+  const Cache8& C = A.C;
+  if (C.cu == nullptr) {
+    const int per = (A.G + kRowsB - 1) / kRowsB;
+    return unit_of(A, seq8(C, u / per), u % per * kRowsB);
+  }
+  const Found8 f = find8_scalar(C, u, [&](int c0, int64_t b) { return (int64_t)c0 * A.G / kRowsB + b; });
+  return unit_of(A, f.s, max(u - f.first, (int64_t)0) * kRowsB);
 }
 
 // The positions that a query row sees: up to `upto`, and before `sink` or from
@@ -1259,17 +1264,83 @@ constexpr int kSegs = kTileB / 16;                  // 16-token segments of a ti
 static_assert(kChunkB * kSegs == kThreadsB, "a thread a segment");
 static_assert(kThreadsA == kThreadsB, "one launch for both kernels");
 
-// The workspace behind the narrow kernel's: partial rows, and their sums.
-__device__ __forceinline__ float* wide_rows(const Attn8Args& A) { return A.part + A.wide_at; }
-__device__ __forceinline__ float* wide_sums(const Attn8Args& A) {
-  return wide_rows(A) + A.units * A.C.KVH * A.splits * kRowsB * kHeadDim;
+// Where the units are too few to fill the GPU, their tiles are dealt to the
+// workgroups in parts of equal size, as the lengths on the device make it: with
+// `few` workgroups a KV head, parts of all tiles / (few - units), so that the
+// parts that are not whole still find a workgroup each (a sequence's units count
+// as having the tiles of its last), or smaller ones if they do too.  Every
+// workgroup makes the same deal, and takes the part of its number.  (As many
+// parts of each unit, whatever its length: 8 sequences of up to 4000 tokens with
+// 5 new ones each 32 us, so 26; more workgroups than fill the GPU: no gain.)
+struct DealB {
+  Unit8 U;
+  int ordinal, units;    // the unit's place among those with rows, and their number
+  int first, split, splits;
+};
+__device__ __forceinline__ bool deal_b(const Attn8Args& A, int slot, int lane, DealB& d) {
+  const Cache8& C = A.C;
+  const int64_t seqs = C.B + (C.cu != nullptr);   // (with the rows past the last sequence)
+  uint32_t units = 0, tiles = 0;
+  Seq8 s;
+  auto take = [&](int64_t b) {
+    s = b < seqs ? seq8(C, b) : Seq8{0, 0, 0, 0};
+    units = (uint32_t)((rows_b(A, s) + kRowsB - 1) / kRowsB);
+    tiles = units ? (uint32_t)unit_of(A, s, (int64_t)(units - 1) * kRowsB).tiles() : 0u;
+  };
+  uint64_t all = 0;
+  d.units = 0;
+  for (int64_t b0 = (seqs - 1) & ~(int64_t)63; b0 >= 0; b0 -= 64) {
+    take(b0 + lane);
+    const uint64_t mine = (uint64_t)units * tiles;
+    all += last_lane(upto_lane((uint32_t)mine & 0xffffu)) + ((uint64_t)last_lane(upto_lane((uint32_t)(mine >> 16))) << 16);
+    d.units += (int)last_lane(upto_lane(units));
+  }
+  const uint32_t parts = (uint32_t)max(A.few - d.units, (A.few + 1) / 2);
+  uint32_t per = all >> 31 ? (uint32_t)about((int64_t)all, parts) : max(up((uint32_t)all, parts), 4u);
+  if (seqs <= 64 && all >> 31 == 0) {   // or less, if that does too
+    const uint32_t even = max(up((uint32_t)all, (uint32_t)A.few), 4u), more = per - min(even, per);
+#pragma unroll
+    for (int k = 3; k >= 0; --k) {
+      const uint32_t t = even + (more * k >> 2);
+      if (t < per && (int)last_lane(upto_lane(units * max(up(tiles, t), 1u))) <= A.few) per = t;
+    }
+  }
+  int base = 0, before = 0;
+  for (int64_t b0 = 0;;) {
+    const uint32_t splits = max(up(tiles, per), 1u), mine = units * splits, upto = upto_lane(mine), counts = upto_lane(units);
+    const uint64_t past = __ballot(base + (int)upto > slot);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      d.splits = __builtin_amdgcn_readlane((int)splits, at);
+      const int into = slot - base - __builtin_amdgcn_readlane((int)(upto - mine), at), nth = into / d.splits;
+      d.split = into - nth * d.splits;
+      d.first = slot - d.split;
+      d.ordinal = before + __builtin_amdgcn_readlane((int)(counts - units), at) + nth;
+      s = Seq8{__builtin_amdgcn_readlane(s.b, at), __builtin_amdgcn_readlane(s.c0, at),
+               __builtin_amdgcn_readlane(s.n, at), __builtin_amdgcn_readlane(s.len, at)};
+      d.U = unit_of(A, s, (int64_t)nth * kRowsB);
+      return true;
+    }
+    base += (int)last_lane(upto);
+    before += (int)last_lane(counts);
+    b0 += 64;
+    if (b0 >= seqs) return false;
+    take(b0 + lane);
+  }
 }
 
-// The tiles of split s of a pair.
-__device__ __forceinline__ void split_tiles(const Attn8Args& A, int nt, int s, int& j0, int& j1) {
-  const int per = max((nt + A.splits - 1) / A.splits, 4);
-  j0 = min(s * per, nt);
-  j1 = min(j0 + per, nt);
+// The workspace behind the narrow kernel's: partial rows, their sums, how each
+// unit was left, and (behind the last that can be) the units' number.
+struct LeftB {
+  int first, n;     // slots first .. first + n - 1 have parts of its rows (n = 1: written whole),
+  int row, rows;    // rows row .. row + rows - 1 of the call
+};
+__device__ __forceinline__ float* wide_rows(const Attn8Args& A) { return A.part + A.wide_at; }
+__device__ __forceinline__ float* wide_sums(const Attn8Args& A) {
+  return wide_rows(A) + (int64_t)A.slots * A.C.KVH * kRowsB * kHeadDim;
+}
+__device__ __forceinline__ LeftB* wide_left(const Attn8Args& A) {
+  return reinterpret_cast<LeftB*>(wide_sums(A) + (int64_t)A.slots * A.C.KVH * kRowsB * 2);
 }
 
 struct WideLds {
@@ -1282,8 +1353,11 @@ struct WideLds {
   int nan_seen[4];
 };
 
-template <int CODE, int E>
-__device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideLds& L8) {
+// Tiles [j0, j1) of unit U.  HALF: at most half of kRowsB rows; the waves are two
+// for the rows and each 32 tokens of a tile, joined at the end (32 sequences of up
+// to 4000 tokens with 5 new ones each, 40 rows: 74 -> 57 us).
+template <int CODE, int E, bool HALF>
+__device__ __forceinline__ void wide_tiles(const Attn8Args& A, const Unit8& U, int head, int j0, int j1, WideLds& L8) {
   auto& ks = L8.k;
   auto& vs = L8.v;
   auto& metas = L8.metas;
@@ -1293,21 +1367,11 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
   const Cache8& C = A.C;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
-  // KV heads fastest (they go to different XCDs' caches), then splits; the last
-  // rows of a sequence, which have the most tiles, first
-  const int head = (int)(id % (uint32_t)C.KVH);
-  id /= (uint32_t)C.KVH;
-  const int split = (int)(id % (uint32_t)A.splits);
-  const int64_t u = A.units - 1 - (int64_t)(id / (uint32_t)A.splits);
-  const Unit8 U = unit_b(A, u);
-  if (U.rows == 0) return;
-  const int nt = U.tiles();
-  int j0, j1;
-  split_tiles(A, nt, split, j0, j1);
-  const bool whole = j1 - j0 == nt;
-  if (j0 == j1 && !(whole && split == 0)) return;
+  constexpr int kParts = HALF ? 1 : 2;   // of a tile's tokens, 32 each, that a wave takes,
+  const int b0 = HALF ? wave >> 1 : 0;   // from this one on
+  const bool whole = j1 - j0 == U.tiles();
 
-  const int my_row = 32 * wave + n;
+  const int my_row = 32 * (HALF ? wave & 1 : wave) + n;
   const int my_tok = (U.row0 + my_row) / A.G, my_head = U.row0 + my_row - my_tok * A.G;
   const bool mine = my_row < U.rows;
   const Sight8 sight = sight8(A, U, mine ? U.s.len - U.s.n + my_tok : -1);
@@ -1334,7 +1398,8 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
   const int r16 = 4 * wave + (lane >> 4), ch = lane & 15;
   uint32_t off0 = (uint32_t)r16 * C.row_bytes + 8u * ch;
   uint32_t k_at = r16 * kRowB + ((ch ^ r16) << 4), v_at = r16 * kRowB + ((ch ^ ((r16 & 3) << 2)) << 4);
-  asm volatile("" : "+v"(off0), "+v"(k_at), "+v"(v_at));   // kept, not computed again for each tile
+  uint32_t q_at = n * kRowB + ((hf ^ (n & 15)) << 4);   // row n's chunk 2 s + hf is at q_at ^ (s << 5)
+  asm volatile("" : "+v"(off0), "+v"(k_at), "+v"(v_at), "+v"(q_at));   // kept, not computed again for each tile
 
   for (int i0 = j0; i0 < j1; i0 += kChunkB) {
     const int cnt = min(j1 - i0, kChunkB);
@@ -1416,19 +1481,20 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
       mend(i + 1);
       // this tile's S = K Q^T, and meanwhile the next one staged (past the last:
       // zeros) and the one behind it loaded
-      float16v S[2];
+      float16v S[kParts];
       const char* kt = ks[i & 1];
+      uint32_t now_at = q_at;
+      asm volatile("" : "+v"(now_at));   // (the eight addresses are not kept: their registers are the operands')
       const char* vt = vs[i & 1];
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < kParts; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[b][r] = 0.f;
 #pragma unroll
       for (int s = 0; s < 8; ++s) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-          S[b] = mfma32x32x16<E>(*reinterpret_cast<const u32x4*>(kt + (32 * b + n) * kRowB + (((2 * s + hf) ^ (n & 15)) << 4)),
-                                 qB[s], S[b]);
+        for (int b = 0; b < kParts; ++b)
+          S[b] = mfma32x32x16<E>(*reinterpret_cast<const u32x4*>(kt + 32 * (b0 + b) * kRowB + (now_at ^ (s << 5))), qB[s], S[b]);
         if (s & 1) {
           stage_v(i + 1, s >> 1);
           load(i + 2, s >> 1);
@@ -1439,10 +1505,10 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
       {
         // logits against the running maximum (0 while there is none)
         const float ref = m == -INFINITY ? 0.f : m;
-        float inv[kSegs], top = -INFINITY;
+        float inv[2 * kParts], top = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < kSegs; ++g) {
-          const Meta8 mt = metas[kSegs * i + g];
+        for (int g = 0; g < 2 * kParts; ++g) {
+          const Meta8 mt = metas[kSegs * i + 2 * b0 + g];
           inv[g] = mt.inv;
           const float add = mt.lv - ref;
 #pragma unroll
@@ -1452,15 +1518,15 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
         }
         if (!full) {
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
+          for (int b = 0; b < kParts; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              const int p = tok + 32 * b + 8 * (r >> 2) + 4 * hf + (r & 3);
+              const int p = tok + 32 * (b0 + b) + 8 * (r >> 2) + 4 * hf + (r & 3);
               S[b][r] = sight.sees(p) ? S[b][r] : -INFINITY;
             }
         }
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < kParts; ++b)
 #pragma unroll
           for (int r = 0; r < 16; ++r) top = fmaxf(top, S[b][r]);
         if (__any(top > (m == -INFINITY ? -INFINITY : kRescaleSlack))) {
@@ -1470,7 +1536,7 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
           const float f = __builtin_amdgcn_exp2f(m - to);   // 0 while there was none
           const float d = ref - to;
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
+          for (int b = 0; b < kParts; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) S[b][r] += d;
           l *= f;
@@ -1482,10 +1548,10 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
         }
         // lane (group of 16 lanes, 4j + h): row 4 hf + j, channel 16 (group & 1) + 4 h
         const int j = (lane >> 2) & 3;
-        const char* vl = vt + (4 * hf + j) * kRowB + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+        const char* vl = vt + (32 * b0 + 4 * hf + j) * kRowB + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
         // 16 tokens' weights, then their products, under which the next 16's are made
 #pragma unroll
-        for (int g = 0; g < kSegs; ++g) {
+        for (int g = 0; g < 2 * kParts; ++g) {
           half8 h;
           float sum = 0.f;
 #pragma unroll
@@ -1504,7 +1570,7 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
         }
         if (nans) {   // and reaches the rows that do
           u32x4 hit = {0u, 0u, 0u, 0u};   // this row's channels
-          for (int p = 0; p < kTileB; ++p)
+          for (int p = 32 * b0; p < 32 * (b0 + kParts); ++p)
             if (sight.sees(tok + p)) hit |= *reinterpret_cast<const u32x4*>(nan_map[i & 1][p]);
 #pragma unroll
           for (int cb = 0; cb < 4; ++cb) {
@@ -1519,9 +1585,36 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
     }
   }
 
-  if (!mine) return;
   l = half_sum(l);
-  const int64_t at = whole ? out_row(A, U, head, my_row) : (((u * C.KVH + head) * A.splits + split) * kRowsB + my_row) * kHeadDim;
+  if constexpr (HALF) {   // the tokens' halves joined, through what K's tiles were in
+    float4v* const parked = reinterpret_cast<float4v*>(&ks[wave & 1][0]) + lane;
+    float2v* const sums = reinterpret_cast<float2v*>(&vs[wave & 1][0]) + lane;
+    if (b0) {
+#pragma unroll
+      for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+          parked[64 * (4 * cb + r / 4)] = float4v{O[cb][r], O[cb][r + 1], O[cb][r + 2], O[cb][r + 3]};
+      *sums = float2v{m, l};
+    }
+    __syncthreads();
+    if (b0) return;
+    const float2v other = *sums;
+    const float top = fmaxf(m, other[0]), ref = top == -INFINITY ? 0.f : top;
+    const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(other[0] - ref);
+    m = top;
+    l = __builtin_fmaf(l, f0, other[1] * f1);
+#pragma unroll
+    for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const float4v v = parked[64 * (4 * cb + r / 4)];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) O[cb][r + k] = __builtin_fmaf(O[cb][r + k], f0, v[k] * f1);
+      }
+  }
+  if (!mine) return;
+  const int64_t at = whole ? out_row(A, U, head, my_row) : ((int64_t)blockIdx.x * kRowsB + my_row) * kHeadDim;   // (a slot and KV head's)
 #pragma unroll
   for (int cb = 0; cb < 4; ++cb)
 #pragma unroll
@@ -1538,51 +1631,91 @@ __device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideL
   }
 }
 
-// Joins the splits of the wide kernel's rows, 32 threads a row, eight splits on
+template <int CODE, int E>
+__device__ __forceinline__ void wide_part(const Attn8Args& A, uint32_t id, WideLds& L8) {
+  const Cache8& C = A.C;
+  const int lane = threadIdx.x & 63;
+  // KV heads fastest (they go to different XCDs' caches); the last rows of a
+  // sequence, which have the most tiles, first
+  const int head = (int)(id % (uint32_t)C.KVH);
+  id /= (uint32_t)C.KVH;
+  Unit8 U;
+  int j0 = 0, j1;
+  if (A.slots == 0) {
+    U = unit_b(A, A.units - 1 - (int64_t)id);
+    if (U.rows == 0) return;
+    j1 = U.tiles();
+  } else {
+    DealB d;
+    const bool some = deal_b(A, (int)id, lane, d);
+    const bool says = head == 0 && threadIdx.x == 0;
+    if (says && id == 0) wide_left(A)[A.units].n = d.units;
+    if (!some) return;
+    U = d.U;
+    const int nt = U.tiles(), per = max((nt + d.splits - 1) / d.splits, 1);
+    j0 = min(d.split * per, nt);
+    j1 = min(j0 + per, nt);
+    if (says && d.split == 0 && d.ordinal < A.units)
+      wide_left(A)[d.ordinal] = LeftB{d.first, max((nt + per - 1) / per, 1), U.s.c0 * A.G + U.row0, U.rows};
+    if (j0 == j1 && d.split > 0) return;
+  }
+  if (U.rows > kRowsB / 2) {   // (this one first: the other way round its operands are read too late, 6%)
+    wide_tiles<CODE, E, false>(A, U, head, j0, j1, L8);
+    return;
+  }
+  wide_tiles<CODE, E, true>(A, U, head, j0, j1, L8);
+}
+
+// Joins the parts of the wide kernel's rows, 32 threads a row, eight parts on
 // their way.
 template <int E>
 __device__ __forceinline__ void wide_join(const Attn8Args& A, uint32_t block) {
   const Cache8& C = A.C;
-  const int64_t pair = block / (kRowsB / 8);
-  const int row = 8 * (int)(block % (kRowsB / 8)) + (threadIdx.x >> 5), chunk = threadIdx.x & 31;
-  const int64_t u = pair / C.KVH;
-  const int head = (int)(pair - u * C.KVH);
-  const Unit8 U = unit_b(A, u);
-  const int nt = U.tiles();
-  int j0, j1;
-  split_tiles(A, nt, 0, j0, j1);
-  if (row >= U.rows || j1 == nt) return;
-  const int64_t first = pair * A.splits * kRowsB + row;
-  const int splits = (nt + j1 - 1) / j1;
+  const uint32_t per = kRowsB / 8 / A.passes;   // workgroups of a unit and KV head
+  const uint32_t pair = block / per;
+  const int chunk = threadIdx.x & 31, head = (int)(pair % (uint32_t)C.KVH), u = (int)(pair / (uint32_t)C.KVH);
+  const int units = wide_left(A)[A.units].n;
+  LeftB left = wide_left(A)[u];
+  if (u >= units) return;
+  // (inside the workspace and the output whatever it holds)
+  left.first = min(max(left.first, 0), A.slots - 1);
+  left.n = min(left.n, A.slots - left.first);
+  left.row = min(max(left.row, 0), (int)C.T * A.G);
+  left.rows = min(min(left.rows, kRowsB), (int)C.T * A.G - left.row);
+  if (left.n <= 1) return;
   const float2v* sums = reinterpret_cast<const float2v*>(wide_sums(A));
-  float M = -INFINITY, L = 0.f;
-  float4v acc = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < splits; s0 += 8) {
-    float2v ml[8];
-    float4v a[8];
-    float top = M;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int64_t p = first + (int64_t)min(s0 + k, splits - 1) * kRowsB;
-      ml[k] = sums[p];
-      a[k] = *reinterpret_cast<const float4v*>(wide_rows(A) + p * kHeadDim + 4 * chunk);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k][0]);
-    const float ref = top == -INFINITY ? 0.f : top;   // (a row that saw nothing yet)
-    const float again = __builtin_amdgcn_exp2f(M - ref);
-    M = top;
-    acc = acc * again;
-    L *= again;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (s0 + k < splits) {
-        const float f = __builtin_amdgcn_exp2f(ml[k][0] - ref);
-        acc += a[k] * f;
-        L = __builtin_fmaf(ml[k][1], f, L);
+  for (int row = 8 * (int)(block - pair * per) + (int)(threadIdx.x >> 5); row < left.rows; row += 8 * (int)per) {
+    const int64_t first = ((int64_t)left.first * C.KVH + head) * kRowsB + row;
+    float M = -INFINITY, L = 0.f;
+    float4v acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < left.n; s0 += 8) {
+      float2v ml[8];
+      float4v a[8];
+      float top = M;
+  #pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int64_t p = first + (int64_t)min(s0 + k, left.n - 1) * C.KVH * kRowsB;
+        ml[k] = sums[p];
+        a[k] = *reinterpret_cast<const float4v*>(wide_rows(A) + p * kHeadDim + 4 * chunk);
       }
+  #pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k][0]);
+      const float ref = top == -INFINITY ? 0.f : top;   // (a row that saw nothing yet)
+      const float again = __builtin_amdgcn_exp2f(M - ref);
+      M = top;
+      acc = acc * again;
+      L *= again;
+  #pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (s0 + k < left.n) {
+          const float f = __builtin_amdgcn_exp2f(ml[k][0] - ref);
+          acc += a[k] * f;
+          L = __builtin_fmaf(ml[k][1], f, L);
+        }
+    }
+    const int r = left.row + row, tok = r / A.G;
+    store_out<E>(A, ((int64_t)tok * A.H + head * A.G + (r - tok * A.G)) * kHeadDim + 4 * chunk, acc, L);
   }
-  store_out<E>(A, out_row(A, U, head, row) + 4 * chunk, acc, L);
 }
 
 // ---- launches ----
@@ -1729,28 +1862,30 @@ int narrow_side(int32_t KVH) { return KVH % 4 == 0 ? 4 : KVH % 2 == 0 ? 2 : 1; }
 constexpr int kManyPairs = 64;   // from here on the pairs' parts are few (eight or so)
 
 // Wide kernel: units of a call (with those of the rows past the last sequence),
-// and splits a pair where the pairs do not fill the GPU.
+// and slots a KV head where the units do not fill the GPU (no part is of less
+// than 4 tiles).
 int64_t wide_units(bool offsets, int64_t B, int64_t T, int32_t G) {
   if (!offsets) return G > kRowsA ? B * ((G + kRowsB - 1) / kRowsB) : 0;
   return T * G / kRowsB + B + 1;
 }
-int wide_splits(int64_t units, int32_t KVH, int64_t max_len) {
-  const int64_t pairs = std::max<int64_t>(units * KVH, 1), tiles = (max_len + kTileB - 1) / kTileB;
-  return (int)std::max<int64_t>(1, std::min((kPairsB + pairs - 1) / pairs, tiles / 4));
+int wide_slots(int64_t units, int32_t KVH, int64_t max_len) {
+  const int64_t tiles = (max_len + kTileB - 1) / kTileB;
+  if (units * KVH >= kPairsB || tiles <= 4) return 0;
+  return (int)std::min(kPairsB / KVH + units, units * ((tiles + 3) / 4));
 }
-size_t wide_bytes(int64_t units, int32_t KVH, int splits) {
-  return splits <= 1 ? 0 : (size_t)units * KVH * splits * kRowsB * (kHeadDim + 2) * sizeof(float);
+size_t wide_bytes(int64_t units, int32_t KVH, int slots) {
+  return slots == 0 ? 0 : (size_t)slots * KVH * kRowsB * (kHeadDim + 2) * sizeof(float) + (size_t)(units + 1) * sizeof(LeftB);
 }
 
 size_t attn_bytes(bool offsets, int64_t B, int64_t T, int32_t G, int32_t KVH, int64_t max_len) {
   const int64_t units = wide_units(offsets, B, T, G);
   return narrow_bytes(narrow_groups(B, KVH, G, max_len), narrow_side(KVH), B * KVH) +
-         wide_bytes(units, KVH, wide_splits(units, KVH, max_len));
+         wide_bytes(units, KVH, wide_slots(units, KVH, max_len));
 }
 
 template <int CODE, int E>
 int launch_attn8(Attn8Args A, hipStream_t stream) {
-  const unsigned wide = (unsigned)(A.units * A.C.KVH * A.splits);
+  const unsigned wide = (unsigned)((A.slots ? A.slots : A.units) * A.C.KVH);
   if (A.groups == 0)
     wide8_kernel<CODE, E><<<dim3(wide), dim3(kThreadsB), 0, stream>>>(A);
   else if (wide == 0)
@@ -1759,7 +1894,9 @@ int launch_attn8(Attn8Args A, hipStream_t stream) {
     both8_kernel<CODE, E><<<dim3(wide + A.groups), dim3(kThreadsB), 0, stream>>>(A);
   const int rc = launch_status();
   if (rc) return rc;
-  A.wide_blocks = A.splits > 1 ? (unsigned)(A.units * A.C.KVH * (kRowsB / 8)) : 0;
+  A.passes = 1;
+  while (A.passes < kRowsB / 8 && A.units * A.C.KVH * (kRowsB / 8) / A.passes > kJoinsB) A.passes *= 2;
+  A.wide_blocks = A.slots ? (unsigned)(A.units * A.C.KVH * (kRowsB / 8) / A.passes) : 0;
   const int64_t heads = A.groups ? A.C.B * A.C.KVH : 0;
   if (heads / A.side >= kManyPairs)
     join8_kernel<E, true><<<dim3(A.wide_blocks + (unsigned)heads), dim3(256), 0, stream>>>(A);
@@ -1837,8 +1974,9 @@ int kvdec_paged8_attention(const kvdec_paged8_cache* cache, const void* q, void*
   A.pairs = A.C.KVH / A.side;
   A.inv_g = (uint32_t)((65536 + A.G - 1) / A.G);
   A.units = wide_units(offsets, B, T, A.G);
-  A.splits = wide_splits(A.units, A.C.KVH, A.C.max_len);
-  if (B * A.C.KVH * kRowsA + A.units * A.C.KVH * std::max(A.splits, kRowsB / 8) + A.groups > 0x7fffffff)
+  A.slots = wide_slots(A.units, A.C.KVH, A.C.max_len);
+  A.few = kPairsB / A.C.KVH;
+  if (B * A.C.KVH * kRowsA + A.units * A.C.KVH + 16 * kPairsB + A.groups > 0x7fffffff)
     return KVDEC_E_SHAPE;
   if (!ws || !on16(ws) || ws_bytes < attn_bytes(offsets, B, T, A.G, A.C.KVH, A.C.max_len)) return KVDEC_E_WORKSPACE;
   A.q = q;

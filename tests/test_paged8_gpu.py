@@ -466,6 +466,46 @@ def test_attend_many_sequences(device):
     check_out(o2, ref, "fp16", vmax_of(c, "int8"))
 
 
+# sequences, length of the others, (H, KVH), new tokens a sequence (None: one each, no offsets), window, sink
+DEALT = [(140, 330, (8, 1), "draft", None, 0),      # three waves' lanes of sequences, 64-row units
+         (3, 2500, (8, 2), "draft", None, 0),       # few long ones: many parts each
+         (70, 700, (33, 1), None, None, 0),         # one token each, of more rows than the narrow kernel's
+         (40, 900, (8, 1), "chunk", None, 0),       # units of 128 and of 64 rows, several a sequence
+         (9, 1500, (16, 2), "chunk", 200, 70),
+         (20, 300, (8, 8), "chunk", None, 0)]
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("case", range(len(DEALT)))
+def test_attend_dealt_units(code, case, device):
+    """Units too few to fill the GPU, whose tiles are dealt in parts: ragged
+    lengths, empty sequences among them, and rows of no sequence."""
+    from paged8_kernel import paged8_attention
+    B, length, (H, KVH), kind, window, sink = DEALT[case]
+    rng = np.random.default_rng(60 + case)
+    ps = 16
+    lens = [int(n) for n in rng.integers(0, length, B)]
+    lens[0], lens[B // 2], lens[-1] = 2 * length, 0, 1
+    new = [1] * B
+    if kind == "draft":
+        new = [int(n) for n in rng.integers(0, 9, B)]
+    if kind == "chunk":
+        new = [int(n) for n in np.where(rng.random(B) < 0.3, rng.integers(0, 60, B), 1)]
+        new[0] = 33
+    T = sum(new) + (0 if kind is None else 3)
+    c = make_cache(rng, sum(-(-n // ps) for n in lens) + 1, KVH, ps, 16, code, "NHD")
+    table, cu = make_table(rng, lens, ps, len(c["k_pages"])), None if kind is None else np.cumsum([0] + new)
+    q = torch.from_numpy(rng.standard_normal((T, H, D)).astype(np.float32)).half()
+    ref = O.attention(q.double().numpy(), c, table, lens, cu, SCALE, code, window=window, sink=sink)
+    say(f"dealt units {code} {DEALT[case]}")
+    args = (q.to(device), *put(c, code, device), i32(table, device), i32(lens, device), i32(cu, device))
+    o = paged8_attention(*args, window=window, sink=sink)
+    again = paged8_attention(*args, window=window, sink=sink)
+    torch.cuda.synchronize()
+    check_out(o, ref, "fp16", vmax_of(c, code), single=True)
+    assert torch.equal(o, again)
+
+
 def test_pool_past_4_gib(device):
     """Page offsets past 32 bits, in codes and in scales."""
     from paged8_kernel import new_paged8_cache, paged8_attention, read_paged8_cache, write_paged8_cache
