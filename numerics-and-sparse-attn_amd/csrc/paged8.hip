@@ -535,6 +535,10 @@ struct Unit8 {
   __device__ __forceinline__ int tile(int j) const { return j < ts ? j : tw + j - ts; }
 };
 
+// The first position of a window that ends at `pos` (any window up to INT32_MAX,
+// and positions before the start, which see nothing).
+__device__ __forceinline__ int from8(const Attn8Args& A, int pos) { return max(pos, -1) - A.window + 1; }
+
 template <int TILE>
 __device__ __forceinline__ void unit_tiles(const Attn8Args& A, Unit8& U, int pos0, int pos1) {
   U.ts = U.tw = U.te = U.hi = 0;
@@ -550,7 +554,7 @@ __device__ __forceinline__ void unit_tiles(const Attn8Args& A, Unit8& U, int pos
   U.te = (U.hi + TILE - 1) / TILE;
   if (A.window > 0) {
     U.ts = min((int)(((int64_t)A.sink + TILE - 1) / TILE), U.te);
-    U.tw = min(max(U.ts, max(U.pos0 - A.window + 1, 0) / TILE), U.te);
+    U.tw = min(max(U.ts, max(from8(A, U.pos0), 0) / TILE), U.te);
   }
 }
 
@@ -611,7 +615,7 @@ struct Sight8 {
   __device__ __forceinline__ bool sees(int p) const { return (p <= upto) & ((p < sink) | (p >= from)); }
 };
 __device__ __forceinline__ Sight8 sight8(const Attn8Args& A, const Unit8& U, int pos) {
-  return A.window > 0 ? Sight8{min(pos, U.hi - 1), pos - A.window + 1, A.sink} : Sight8{min(pos, U.hi - 1), 0, 0};
+  return A.window > 0 ? Sight8{min(pos, U.hi - 1), from8(A, pos), A.sink} : Sight8{min(pos, U.hi - 1), 0, 0};
 }
 
 // Every token of [tok, tok + n) is seen by every row of the unit.
@@ -885,7 +889,7 @@ __device__ __forceinline__ void narrow_part(const Attn8Args& A, int group, Narro
     st.m = kMaxSentinel;
     st.l = 0.f;
 
-    const int hi = U.hi, lo = A.window > 0 ? max(U.pos0 - A.window + 1, 0) : 0;
+    const int hi = U.hi, lo = A.window > 0 ? max(from8(A, U.pos0), 0) : 0;
     const int sink = A.window > 0 ? A.sink : 0;
     const char* kbase = C.k + head * C.head_bytes;
     const char* vbase = C.v + head * C.head_bytes;
@@ -1410,7 +1414,7 @@ __device__ __forceinline__ void wide_tiles(const Attn8Args& A, const Unit8& U, i
     for (int r = 0; r < 16; ++r) O[cb][r] = 0.f;
   float m = -INFINITY, l = 0.f;   // no token seen yet; the lane's share of the sum
 
-  const int hi = U.hi, lo = A.window > 0 ? max(U.pos0 - A.window + 1, 0) : 0;
+  const int hi = U.hi, lo = A.window > 0 ? max(from8(A, U.pos0), 0) : 0;
   const int sink = A.window > 0 ? A.sink : 0;
   const char* kbase = C.k + head * C.head_bytes;
   const char* vbase = C.v + head * C.head_bytes;

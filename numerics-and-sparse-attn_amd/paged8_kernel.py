@@ -41,6 +41,7 @@ import _kvdec as K
 _LAYOUTS = ("NHD", "HND")
 _CODES = {torch.int8: K.I8, torch.float8_e4m3fn: K.E4M3}
 _MAX_LEN = 2**30   # tokens of a block-table row, less than this
+_MAX_INT = 2**31 - 1
 
 
 def new_paged8_cache(num_pages, n_kv_heads=N_KV_HEADS, page_size=64, block_size=32, dtype=torch.float8_e4m3fn,
@@ -226,6 +227,7 @@ def paged8_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, seq_l
     window, sink = (None if window is None else int(window)), int(sink)
     if sink < 0 or (sink > 0 if window is None else window < 1):
         raise ValueError(f"window must be None or >= 1, and sink >= 0 (0 without a window), got {window} and {sink}")
+    window, sink = min(window or 0, _MAX_INT), min(sink, _MAX_INT)   # positions end before that
     o = torch.empty((T, H, D_HEAD), dtype=q.dtype, device=q.device)
     if B == 0 or o.numel() == 0:
         return o.zero_()
@@ -235,7 +237,7 @@ def paged8_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, seq_l
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     with torch.cuda.device(q.device):
         rc = K.lib.kvdec_paged8_attention(ctypes.byref(c), K.ptr(q), K.ptr(o), _checks.ATTN_DTYPES[q.dtype],
-                                          q.stride(0), q.stride(1), K.ptr(cu_seqlens), B, T, H, window or 0, sink,
+                                          q.stride(0), q.stride(1), K.ptr(cu_seqlens), B, T, H, window, sink,
                                           float(sm_scale), K.ptr(ws), nbytes, K.stream_of(q))
     K.check(rc, "paged8_attention")
     return o

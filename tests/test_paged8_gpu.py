@@ -446,6 +446,30 @@ def test_attend_past_the_table(many, window, device):
     check_out(o, ref, "fp16", vmax_of(c, "int8"), single=many)
 
 
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("window, sink", [(2**31 - 1, 0), (2**31 - 40, 3), (2**31, 1), (2**32 + 1, 0), (5, 2**31 - 1),
+                                          (5, 2**32 + 3), (2**70, 2**70)])
+def test_attend_windows_of_any_size(window, sink, many, device):
+    """Windows and sinks at and past the ends of 32 bits, also of sequences with
+    more new tokens than length."""
+    from paged8_kernel import paged8_attention
+    rng = np.random.default_rng(58)
+    H, KVH, ps = 4, 2, 16
+    lens = [70, 3, 1, 20, 90]
+    new = [2, 6, 8, 60, 1] if many else [1] * 5
+    c = make_cache(rng, 20, KVH, ps, 16, "e4m3", "NHD")
+    table = make_table(rng, lens, ps, 20)
+    cu = np.cumsum([0] + new) if many else None
+    q = torch.from_numpy(rng.standard_normal((sum(new), H, D)).astype(np.float32)).half()
+    # every position is within 100 of the others: so is what the oracle is given
+    ref = O.attention(q.double().numpy(), c, table, lens, cu, SCALE, "e4m3", window=min(window, 100), sink=min(sink, 100))
+    say(f"windows of any size W {window} S {sink} many {many}")
+    o = paged8_attention(q.to(device), *put(c, "e4m3", device), i32(table, device), i32(lens, device), i32(cu, device),
+                         window=window, sink=sink)
+    torch.cuda.synchronize()
+    check_out(o, ref, "fp16", vmax_of(c, "e4m3"), single=many)
+
+
 def test_attend_many_sequences(device):
     """More sequences than a wave has lanes, most of them short or empty."""
     from paged8_kernel import paged8_attention
