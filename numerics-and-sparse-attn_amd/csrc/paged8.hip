@@ -490,8 +490,16 @@ __global__ __launch_bounds__(64 * kWriteWaves) void read8_kernel(Read8Args A) {
 // Softmax over scaled codes.  With x = log2(e) sm_scale (q . k) per token, the
 // scale of V's block enters as x + log2(vs): w = exp2(x + log2(vs) - m) is the
 // token's weight times vs, so the product with the codes needs no scale, and
-// the sum of the weights takes w / vs.  m is the running maximum of
-// x + log2(vs), so that w stays in fp16's range whatever the scales.
+// the sum of the weights takes w / vs.  m follows the running maximum of
+// x + log2(vs), so that w stays in fp16's range whatever the scales: it is
+// kLift below the maximum that it was last set from, and set again once that is
+// kHighest above it (8 rather than 15 costs the wide kernel 3%).  fp16 rounds a w
+// to steps of no less than 2^-24, which the lift makes 2^-31 of the largest: where
+// one token outweighs a long cache of equal ones, those are off by no more than
+// 2^-32 each.  The sum is kDown of that, so that 2^19 tokens of the largest weight
+// and the least V scale, 2^-100, stay under 2^128.
+
+constexpr float kLift = 7.f, kHighest = 15.f, kDown = 0x1p-7f;
 
 constexpr int kRowsA = 16;
 constexpr int kWavesA = 4;
@@ -624,7 +632,7 @@ __device__ __forceinline__ bool all_seen(const Attn8Args& A, const Unit8& U, int
 }
 
 // What a token of the pair's rows weighs by: kf turns q . k into x, lv is
-// log2 of V's scale and inv its inverse.  No page: keys and values of zero.
+// log2 of V's scale and inv its inverse (times kDown).  No page: keys and values of zero.
 struct Meta8 {
   int page;
   float kf, lv, inv;
@@ -648,7 +656,7 @@ __device__ __forceinline__ float2v scales8(const Cache8& C, int page, int head, 
 __device__ __forceinline__ Meta8 meta8(const Attn8Args& A, int page, float2v s) {
   const float vs = s[1] < 0x1p-100f ? 0x1p-100f : s[1];   // a scale that is hardly one counts as the writer's least
   return Meta8{page, s[0] * A.scale_log2, __builtin_amdgcn_logf(vs),
-               vs == vs ? 1.f / vs : 1.f};                // a NaN arrives through lv, where masks hold
+               vs == vs ? kDown / vs : 1.f};              // a NaN arrives through lv, where masks hold
 }
 
 // Place of row `row` of a pair in the output.
@@ -659,8 +667,10 @@ __device__ __forceinline__ int64_t out_row(const Attn8Args& A, const Unit8& U, i
 
 template <int E>
 __device__ __forceinline__ void store_out(const Attn8Args& A, int64_t at, float4v acc, float l) {
-  const float d = l == 0.f ? 1.f : l;
-  *reinterpret_cast<u32x2*>((uint16_t*)A.o + at) = round_elt4<E>(float4v{acc[0] / d, acc[1] / d, acc[2] / d, acc[3] / d});
+  // one division for all channels (and a 1 / l that stays finite): whole prompts 1.5%
+  const float up = l < 0x1p-100f ? 0x1p64f : 1.f;
+  const float inv = kDown / (l == 0.f ? 1.f : l * up);
+  *reinterpret_cast<u32x2*>((uint16_t*)A.o + at) = round_elt4<E>(acc * up * inv);
 }
 
 // ---- the narrow kernel ----
@@ -996,23 +1006,27 @@ __device__ __forceinline__ void narrow_part(const Attn8Args& A, int group, Narro
         float top = x[0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-        if (__any(top > st.m + kRescaleSlack)) {
-          const float m = fmaxf(st.m, group_max(top));
+        if (__any(top > st.m + kHighest)) {
+          const float m = fmaxf(st.m, group_max(top) - kLift);
           const float f = __builtin_amdgcn_exp2f(st.m - m);
           st.l *= f;
 #pragma unroll
           for (int cb = 0; cb < 8; ++cb) st.O[cb] = st.O[cb] * f;
           st.m = m;
         }
-        // weights as an fp16 and the fp16 of its remainder: good to 2^-22
+        // weights as an fp16 and the fp16 of its remainder, good to 2^-22 of those
+        // that count; a tile's sum is added at once, so that a long cache of small
+        // ones is not lost beside a large one
         half8 pB, pL;
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float w = __builtin_amdgcn_exp2f(x[j] - st.m);
-          st.l = __builtin_fmaf(w, j < 4 ? inv0 : inv1, st.l);
+          sum[j >> 2] += w;
           pB[j] = (_Float16)w;
           pL[j] = (_Float16)(w - (float)pB[j]);
         }
+        st.l += __builtin_fmaf(sum[0], inv0, sum[1] * inv1);
         const char* vt = slot + kTile * kCodeRow + tau(g, t >> 1) * kCodeRow + 8 * (t & 1);
         if (CODE == kE4m3 && nans) {
           // a NaN reaches the rows that see its token: marked as ones, and
@@ -1506,6 +1520,9 @@ __device__ __forceinline__ void wide_tiles(const Attn8Args& A, const Unit8& U, i
       // this tile's S = K Q^T, and meanwhile the next one staged (past the last:
       // zeros) and the one behind it loaded
       float16v S[kParts];
+      // (ahead of the SIMD's other wave, so that its weights are made under these
+      // products: 2048 new tokens over 8192 519 -> 505 us)
+      __builtin_amdgcn_s_setprio(1);
       const char* kt = ks[i & 1];
       uint32_t now_at = q_at;
       asm volatile("" : "+v"(now_at));   // (the eight addresses are not kept: their registers are the operands')
@@ -1527,6 +1544,7 @@ __device__ __forceinline__ void wide_tiles(const Attn8Args& A, const Unit8& U, i
         }
       }
       {
+        __builtin_amdgcn_s_setprio(0);
         // logits against the running maximum (0 while there is none)
         const float ref = m == -INFINITY ? 0.f : m;
         float inv[2 * kParts], top = -INFINITY;
@@ -1553,8 +1571,8 @@ __device__ __forceinline__ void wide_tiles(const Attn8Args& A, const Unit8& U, i
         for (int b = 0; b < kParts; ++b)
 #pragma unroll
           for (int r = 0; r < 16; ++r) top = fmaxf(top, S[b][r]);
-        if (__any(top > (m == -INFINITY ? -INFINITY : kRescaleSlack))) {
-          const float t = half_max(top);
+        if (__any(top > (m == -INFINITY ? -INFINITY : kHighest))) {
+          const float t = half_max(top) - kLift;
           const float now = m == -INFINITY ? t : fmaxf(m, m + t);
           const float to = now == -INFINITY ? 0.f : now;
           const float f = __builtin_amdgcn_exp2f(m - to);   // 0 while there was none
@@ -1574,6 +1592,7 @@ __device__ __forceinline__ void wide_tiles(const Attn8Args& A, const Unit8& U, i
         const int j = (lane >> 2) & 3;
         const char* vl = vt + (32 * b0 + 4 * hf + j) * kRowB + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
         // 16 tokens' weights, then their products, under which the next 16's are made
+        float part = 0.f;   // a tile's sum, added at once
 #pragma unroll
         for (int g = 0; g < 2 * kParts; ++g) {
           half8 h;
@@ -1584,7 +1603,7 @@ __device__ __forceinline__ void wide_tiles(const Attn8Args& A, const Unit8& U, i
             sum += w;
             h[r] = (_Float16)w;
           }
-          l = __builtin_fmaf(sum, inv[g], l);
+          part = __builtin_fmaf(sum, inv[g], part);
 #pragma unroll
           for (int cb = 0; cb < 4; ++cb) {
             const u32x2 a = lds_read_tr16(vl + 16 * g * kRowB + ((cb ^ j) << 6));
@@ -1592,6 +1611,7 @@ __device__ __forceinline__ void wide_tiles(const Attn8Args& A, const Unit8& U, i
             O[cb] = mfma32x32x16<kEltF16>(u32x4{a[0], a[1], b[0], b[1]}, as_u4(h), O[cb]);
           }
         }
+        l += part;
         if (nans) {   // and reaches the rows that do
           u32x4 hit = {0u, 0u, 0u, 0u};   // this row's channels
           for (int p = 32 * b0; p < 32 * (b0 + kParts); ++p)

@@ -378,6 +378,37 @@ def test_attend_scales_far_apart(code, device):
 
 
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("new", [1, 5])
+def test_one_token_outweighs_many(code, new, device):
+    """A long cache of equal keys beside one that outweighs each of them by
+    2^24.3 and all of them by 200: rounded weights of theirs must not add up to
+    an error.  Beside half a step of fp16 under 1 (2^-12) the result, whose values
+    are 1 and -1, may be off by
+      the weights' steps, 2^-31 of the largest: 2^-32 of each of 50000 at most,
+      2^-24 for each sum in fp32 that a wave makes beside the one: of the 25000
+      tokens of a wave 32 at a time into the weights' sum and, twice, into the
+      product; with several new tokens of 50000, 32 at a time, 16 a product."""
+    from paged8_kernel import paged8_attention
+    H, KVH, ps, L, B = 8, 1, 64, 100_000, 512     # as many sequences of the same pages as workgroups: long sums
+    blocks = -(-L // ps)
+    one = {"int8": 1, "e4m3": 0x38}[code]         # the code of 1.0
+    kp, vp = np.zeros((blocks, ps, KVH, D), np.uint8), np.full((blocks, ps, KVH, D), one, np.uint8)
+    kp[0, 3], vp[0, 3] = one, one | 0x80 if code == "e4m3" else 0xff
+    c = dict(k_pages=kp, v_pages=vp, k_scales=np.ones((blocks, KVH, ps // 32), np.float32),
+             v_scales=np.ones((blocks, KVH, ps // 32), np.float32))
+    table = np.tile(np.arange(blocks, dtype=np.int32), (B, 1))
+    q = torch.full((B * new, H, D), 24.3 * np.log(2) / (D * SCALE), dtype=torch.float16)
+    x = float(q[0, 0, 0]) * D * SCALE             # the logit of the one
+    say(f"one token outweighs many {code} {new}")
+    o = paged8_attention(q.to(device), *put(c, code, device), i32(table, device), i32([L] * B, device),
+                         i32(new * np.arange(B + 1), device))
+    others = np.array([L - new + i for i in range(new)]) * np.exp(-x)
+    want = np.tile((others - 1) / (others + 1), B)[:, None, None]
+    err = np.abs(o.double().cpu().numpy() - want).max()
+    assert err <= 2.0**-12 + 50000 * 2.0**-32 + 3 * (25000 if new == 1 else 50000) / 32 * 2.0**-24, err
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("window", [None, 24])
 def test_masked_nan_stays_out(code, window, device):
     """NaN where a row does not look (behind the last token, later tokens,
