@@ -684,7 +684,7 @@ __device__ __forceinline__ void store_out(const Attn8Args& A, int64_t at, float4
 // workspace, which a second kernel joins.
 //
 // Bound by memory where runs are long: 32 sequences of 32768 tokens and 8 heads,
-// 2.15 GB, take 341 us with the join's 5 (6.3 TB/s; the same loads alone 6.5).
+// 2.15 GB, take 347 us with the join's 5 (6.2 TB/s; the same loads alone 6.5).
 // Where they are short, by latencies: 2 us to the lengths, 2.4 to deal and to find
 // the run, 2.7 for entries, scales and first tiles, 4 for the join of 8 sequences'
 // windows of 4096 tokens, which take 26 us of which 12 are the tiles' own.
@@ -1261,9 +1261,9 @@ __device__ __forceinline__ void narrow_join(const Attn8Args& A, uint32_t block) 
 // of the kernel's bound.
 //
 // Bound by the issue of its products and of the weights between them: e4m3, 2048
-// new tokens of 64 heads over 8192 take 506 us (481 GFLOP, 950 TFLOP/s; the
+// new tokens of 64 heads over 8192 take 512 us (481 GFLOP, 940 TFLOP/s; the
 // matrix units are busy 45% of the time), int8 prompts of 10501 tokens in 6
-// sequences 484 us (373 GFLOP, 770 TFLOP/s, their masked halves of tiles not
+// sequences 492 us (373 GFLOP, 760 TFLOP/s, their masked halves of tiles not
 // counted).
 
 typedef float float16v __attribute__((ext_vector_type(16)));
