@@ -1995,7 +1995,8 @@ int kvdec_paged8_read(const kvdec_paged8_cache* cache, const int32_t* cu_seqlens
 size_t kvdec_paged8_workspace_bytes(int64_t B, int64_t T, int32_t H, int32_t KVH, int64_t max_len) {
   if (B < 1 || T < 1 || H < 1 || KVH < 1 || H % KVH || max_len < 1 || max_len >= ((int64_t)1 << 30)) return 0;
   if (B >= ((int64_t)1 << 24) || T * (H / KVH) >= ((int64_t)1 << 30)) return 0;
-  return std::max(attn_bytes(true, B, T, H / KVH, KVH, max_len), T == B ? attn_bytes(false, B, T, H / KVH, KVH, max_len) : 0);
+  const size_t one_each = T == B ? attn_bytes(false, B, T, H / KVH, KVH, max_len) : 0;
+  return std::max({attn_bytes(true, B, T, H / KVH, KVH, max_len), one_each, (size_t)16});   // (0 is a refusal)
 }
 
 int kvdec_paged8_attention(const kvdec_paged8_cache* cache, const void* q, void* o, int dtype,

@@ -477,6 +477,27 @@ def test_attend_past_the_table(many, window, device):
     check_out(o, ref, "fp16", vmax_of(c, "int8"), single=many)
 
 
+@pytest.mark.parametrize("H, B", [(33, 3), (33, 300), (8, 600)])
+@pytest.mark.parametrize("many", [False, True])
+def test_attend_short_tables(H, B, many, device):
+    """Tables of few tokens, whose rows no workgroups share: groups of more heads
+    than the narrow kernel's rows, and of fewer."""
+    from paged8_kernel import paged8_attention
+    rng = np.random.default_rng(59)
+    ps = 16
+    lens = [int(n) for n in rng.integers(0, 33, B)]
+    new = [int(n) for n in rng.integers(0, 4, B)] if many else [1] * B
+    c = make_cache(rng, sum(-(-n // ps) for n in lens) + 1, 1, ps, 16, "int8", "NHD")
+    table = make_table(rng, lens, ps, len(c["k_pages"]))
+    cu = np.cumsum([0] + new) if many else None
+    q = torch.from_numpy(rng.standard_normal((sum(new), H, D)).astype(np.float32)).half()
+    ref = O.attention(q.double().numpy(), c, table, lens, cu, SCALE, "int8")
+    say(f"short tables {H} {B} many {many}")
+    o = paged8_attention(q.to(device), *put(c, "int8", device), i32(table, device), i32(lens, device), i32(cu, device))
+    torch.cuda.synchronize()
+    check_out(o, ref, "fp16", vmax_of(c, "int8"), single=True)
+
+
 @pytest.mark.parametrize("many", [False, True])
 @pytest.mark.parametrize("window, sink", [(2**31 - 1, 0), (2**31 - 40, 3), (2**31, 1), (2**32 + 1, 0), (5, 2**31 - 1),
                                           (5, 2**32 + 3), (2**70, 2**70)])
