@@ -71,9 +71,13 @@ struct Found8 {
   Seq8 s;
   int64_t first;
 };
+
+// (Sequence B: the rows past the last.)  Where `first` grows by `each` a sequence
+// and by at most `rows` for all rows of the call, only sequences from
+// (u - rows) / each to u / each can be it.
 template <class First>
-__device__ __forceinline__ Found8 find8(const Cache8& C, int64_t u, int lane, First&& first) {
-  int64_t lo = 0, n = C.B + 1;   // B: the rows past the last sequence
+__device__ __forceinline__ Found8 find8(const Cache8& C, int64_t u, int64_t rows, int each, int lane, First&& first) {
+  int64_t lo = max(u - rows, (int64_t)0) / each, n = min(u / each, C.B) - lo + 1;
   while (n > 64) {
     const int64_t step = (n + 63) / 64, s = lo + lane * step;
     const bool ok = s < lo + n && first(offset8(C, s), s) <= u;
@@ -115,7 +119,7 @@ __device__ __forceinline__ Run8 run8(const Cache8& C, int64_t u, int lane) {
   if (C.cu == nullptr) {
     s = seq8(C, u);
   } else {
-    const Found8 f = find8(C, u, lane, [&](int c0, int64_t b) { return ((int64_t)c0 >> C.blk_log2) + 2 * b; });
+    const Found8 f = find8(C, u, C.T >> C.blk_log2, 2, lane, [&](int c0, int64_t b) { return ((int64_t)c0 >> C.blk_log2) + 2 * b; });
     s = f.s;
     j = u - f.first;
   }
@@ -580,8 +584,8 @@ __device__ __forceinline__ Unit8 unit_a(const Attn8Args& A, int64_t b) { return 
 // The same by halving, on scalars alone (the wide kernel has no registers for the
 // search above: 15% of its time).
 template <class First>
-__device__ __forceinline__ Found8 find8_scalar(const Cache8& C, int64_t u, First&& first) {
-  int64_t lo = 0, hi = C.B;
+__device__ __forceinline__ Found8 find8_scalar(const Cache8& C, int64_t u, int64_t rows, First&& first) {
+  int64_t lo = max(u - rows, (int64_t)0), hi = min(u, C.B);
   while (lo < hi) {
     const int64_t mid = (lo + hi + 1) >> 1;
     if (first(offset8(C, mid), mid) <= u) lo = mid; else hi = mid - 1;
@@ -612,7 +616,7 @@ __device__ __forceinline__ Unit8 unit_b(const Attn8Args& A, int64_t u) {
     const int per = (A.G + kRowsB - 1) / kRowsB;
     return unit_of(A, seq8(C, u / per), u % per * kRowsB);
   }
-  const Found8 f = find8_scalar(C, u, [&](int c0, int64_t b) { return (int64_t)c0 * A.G / kRowsB + b; });
+  const Found8 f = find8_scalar(C, u, C.T * A.G / kRowsB, [&](int c0, int64_t b) { return (int64_t)c0 * A.G / kRowsB + b; });
   return unit_of(A, f.s, max(u - f.first, (int64_t)0) * kRowsB);
 }
 
